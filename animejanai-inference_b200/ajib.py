@@ -291,6 +291,124 @@ class Exec:
 
 
 # ---------------------------------------------------------------------------------------------
+# attention operators (aji_b200.h: ajib_rotary_*, ajib_qk_launch, ajib_attention_*). As for the
+# convolutions, launches return the status code; the op holds raw device addresses.
+
+F16, BF16 = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS = 0, 1, 2, 3
+NORM_NONE, NORM_RMS, NORM_L2 = 0, 1, 2
+BIAS_NONE, BIAS_SLOPE, BIAS_TABLE = 0, 1, 2
+
+
+class Heads(C.Structure):
+    """struct ajib_heads: a tensor of heads (address and element strides of sequence, token, head)."""
+    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64), ("sh", C.c_int64)]
+
+
+class RotaryParams(C.Structure):
+    """struct ajib_rotary_params."""
+    _fields_ = [("dim", C.c_int), ("layout", C.c_int), ("axes", C.c_int), ("grid_w", C.c_int), ("scaling", C.c_int),
+                ("base", C.c_double), ("factor", C.c_double), ("trained", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("amplitude", C.c_double), ("freq", C.POINTER(C.c_double))]
+
+
+class QkOp(C.Structure):
+    """struct ajib_qk."""
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("tokens", C.c_int), ("hq", C.c_int), ("hk", C.c_int),
+                ("d", C.c_int), ("rotary", C.c_void_p), ("norm", C.c_int), ("eps", C.c_float), ("wq", C.c_void_p),
+                ("wk", C.c_void_p), ("pos", C.c_void_p), ("pos_sb", C.c_int64), ("pos0", C.c_int), ("len", C.c_void_p)]
+
+
+class AttnOp(C.Structure):
+    """struct ajib_attn."""
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("lq", C.c_int), ("lk", C.c_int), ("hq", C.c_int),
+                ("hk", C.c_int), ("d", C.c_int), ("scale", C.c_float), ("cap", C.c_float), ("causal", C.c_int),
+                ("left", C.c_int), ("right", C.c_int), ("align_end", C.c_int), ("q_len", C.c_void_p),
+                ("k_len", C.c_void_p), ("prefix", C.c_void_p), ("q_doc", C.c_void_p), ("k_doc", C.c_void_p),
+                ("doc_rows", C.c_int), ("bias", C.c_int), ("bias_data", C.c_void_p), ("grid_w", C.c_int),
+                ("reach_y", C.c_int), ("reach_x", C.c_int)]
+
+
+lib.ajib_rotary_create.argtypes = [C.POINTER(RotaryParams), C.POINTER(_vp)]
+lib.ajib_rotary_create.restype = C.c_int
+lib.ajib_rotary_release.argtypes = [C.POINTER(_vp)]
+lib.ajib_rotary_release.restype = None
+lib.ajib_rotary_table.argtypes = [_vp, C.POINTER(C.c_double), C.c_int, C.POINTER(C.c_double)]
+lib.ajib_rotary_table.restype = C.c_int
+lib.ajib_qk_launch.argtypes = [C.POINTER(QkOp), C.POINTER(Heads), C.POINTER(Heads), C.POINTER(Heads), C.POINTER(Heads),
+                               _vp]
+lib.ajib_qk_launch.restype = C.c_int
+lib.ajib_attention_workspace.argtypes = [C.POINTER(AttnOp)]
+lib.ajib_attention_workspace.restype = C.c_size_t
+lib.ajib_attention_launch.argtypes = [C.POINTER(AttnOp), C.POINTER(Heads), C.POINTER(Heads), C.POINTER(Heads),
+                                      C.POINTER(Heads), _vp, C.c_size_t, _vp]
+lib.ajib_attention_launch.restype = C.c_int
+
+
+def heads(ptr, sb, st, sh):
+    """Component i of head h of token t of sequence b at ptr + 2 * (b * sb + t * st + h * sh + i)."""
+    return Heads(ptr, sb, st, sh)
+
+
+class Rotary:
+    """A rotary table (ajib_rotary_create); freq: angles per position that replace base and scaling."""
+
+    def __init__(self, dim, layout=ROTARY_HALF, axes=1, grid_w=0, scaling=ROTARY_PLAIN, base=10000.0, factor=1.0,
+                 trained=0.0, beta_fast=0.0, beta_slow=0.0, amplitude=0.0, freq=None):
+        p = RotaryParams(dim, layout, axes, grid_w, scaling, base, factor, trained, beta_fast, beta_slow, amplitude, None)
+        if freq is not None:
+            if axes not in (1, 2) or len(freq) != dim // 2 // axes:
+                raise AjibError(f"ajib_rotary_create: {len(freq)} frequencies for dim {dim} over {axes} axes")
+            p.freq = (C.c_double * len(freq))(*freq)
+        self.handle = _vp()
+        check(lib.ajib_rotary_create(C.byref(p), C.byref(self.handle)), "ajib_rotary_create")
+
+    def table(self):
+        """(frequencies, amplitude)"""
+        n = lib.ajib_rotary_table(self.handle, None, 0, None)
+        f, a = (C.c_double * n)(), C.c_double()
+        lib.ajib_rotary_table(self.handle, f, n, C.byref(a))
+        return list(f), a.value
+
+    def __del__(self):
+        try:
+            lib.ajib_rotary_release(C.byref(self.handle))
+        except Exception:
+            pass
+
+
+def qk_op(dtype, batch, tokens, hq, hk, d, rotary=None, norm=NORM_NONE, eps=1e-6, wq=0, wk=0, pos=0, pos_sb=None,
+          pos0=0, len_=0):
+    """pos: address of int32 positions, pos_sb apart from sequence to sequence (None: tokens)."""
+    op = QkOp(dtype, batch, tokens, hq, hk, d, None if rotary is None else rotary.handle, norm, eps, wq, wk, pos,
+              tokens if pos_sb is None else pos_sb, pos0, len_)
+    op._rotary = rotary  # keep the table alive as long as the op
+    return op
+
+
+def qk(op, q, k, q_out, k_out, stream=0):
+    """Norm and / or rotation of queries and keys (ajib_qk_launch); Heads, k and k_out None with hk 0."""
+    return lib.ajib_qk_launch(op, q, k, q_out, k_out, stream)
+
+
+def attn_op(dtype, batch, lq, lk, hq, hk, d, scale, cap=0.0, causal=False, left=-1, right=-1, align_end=False, q_len=0,
+            k_len=0, prefix=0, q_doc=0, k_doc=0, doc_rows=0, bias=BIAS_NONE, bias_data=0, grid_w=0, reach_y=0, reach_x=0):
+    return AttnOp(dtype, batch, lq, lk, hq, hk, d, scale, cap, int(causal), left, right, int(align_end), q_len, k_len,
+                  prefix, q_doc, k_doc, doc_rows, bias, bias_data, grid_w, reach_y, reach_x)
+
+
+def attention_workspace(op):
+    """Bytes of device memory a launch of op needs on the current device."""
+    return lib.ajib_attention_workspace(C.byref(op))
+
+
+def attention(op, q, k, v, out, workspace=0, workspace_bytes=0, stream=0):
+    """Attention (ajib_attention_launch) on Heads."""
+    return lib.ajib_attention_launch(op, q, k, v, out, workspace, workspace_bytes, stream)
+
+
+# ---------------------------------------------------------------------------------------------
 # the video ABI (include/aji.h)
 
 AJI_API_VERSION = 9

@@ -1,0 +1,188 @@
+/*
+ * attention.cuh — what the attention kernels share: the arguments, which keys a query sees, the
+ * score, and one row of attention by one warp.
+ *
+ * With scores s_j over the keys a query sees, out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m) for
+ * any m; the kernels keep m = the running maximum and rescale sums by e^(m_old - m_new) when it
+ * grows, so one pass over keys and values suffices. Exponentials are base 2: scores are kept as
+ * s * log2(e), folded into the scale, the cap and the bias.
+ */
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "../../include/aji_b200.h"
+
+namespace ajib {
+
+struct AttnDev {
+    const void *q, *k, *v;
+    void *out;
+    int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
+    int batch, lq, lk, hq, hk, group, d;
+    float scale, cap_in, cap_out;  // s2 = q.k * scale, or cap_out * tanh(q.k * cap_in)
+    int left, right;               // INT_MAX / 2: no limit
+    int align_end;
+    const int *q_len, *k_len, *prefix, *q_doc, *k_doc;
+    int doc_rows, bias;
+    const float *bias_data;
+    int grid_w, reach_y, reach_x;
+    int masked;  // some query may not see some key below its k_len
+};
+
+namespace dev {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// tanh to about 2^-22 of 1: 1 - 2 / (e^2x + 1). (The hardware's tanh.approx is good to 2^-11, which
+// a cap of 50 would turn into 0.02 of score, 2 % of a probability.)
+__device__ __forceinline__ float tanh_exp(float x) { return 1.f - 2.f * rcp_fast(exp2_fast(x * (2.f * kLog2e)) + 1.f); }
+
+// How many queries / keys sequence b has.
+__device__ __forceinline__ int q_count(const AttnDev &p, int b)
+{
+    return p.q_len ? min(max(__ldg(p.q_len + b), 0), p.lq) : p.lq;
+}
+__device__ __forceinline__ int k_count(const AttnDev &p, int b)
+{
+    return p.k_len ? min(max(__ldg(p.k_len + b), 0), p.lk) : p.lk;
+}
+
+// What one query of one head needs to know about every key.
+struct Query {
+    int at;      // its place
+    int lo, hi;  // sees keys lo..hi (both included) and those below pre
+    int pre;
+    int doc;     // INT_MIN: no documents
+    int y, x;    // place on the grid (TABLE)
+    float slope; // SLOPE, times log2(e)
+    const float *table;
+};
+
+__device__ __forceinline__ Query query_of(const AttnDev &p, int b, int h, int i, int qn, int kn)
+{
+    Query r;
+    r.at = i + (p.align_end ? kn - qn : 0);
+    r.lo = p.left == INT_MAX / 2 ? INT_MIN : r.at - p.left;
+    r.hi = p.right == INT_MAX / 2 ? INT_MAX : r.at + p.right;
+    r.pre = p.prefix ? __ldg(p.prefix + b) : 0;
+    r.doc = INT_MIN;
+    if (p.q_doc) {
+        r.doc = i < p.lq ? __ldg(p.q_doc + (int64_t)(b % p.doc_rows) * p.lq + i) : -1;
+        if (r.doc < 0) r.lo = INT_MAX, r.hi = r.pre = INT_MIN;  // padding sees nothing
+    }
+    r.y = 0;
+    r.x = r.at;
+    r.slope = 0.f;
+    r.table = nullptr;
+    if (p.bias == AJIB_BIAS_SLOPE) r.slope = __ldg(p.bias_data + h) * kLog2e;
+    if (p.bias == AJIB_BIAS_TABLE) {
+        if (p.grid_w) {
+            r.y = r.at / p.grid_w;
+            r.x = r.at - r.y * p.grid_w;
+        }
+        r.table = p.bias_data + (int64_t)h * (2 * p.reach_y + 1) * (2 * p.reach_x + 1);
+    }
+    return r;
+}
+
+__device__ __forceinline__ bool in_reach(const Query &r, int j) { return j < r.pre || (j >= r.lo && j <= r.hi); }
+
+__device__ __forceinline__ float table_bias(const AttnDev &p, const Query &r, int jy, int jx)
+{
+    const int dy = min(max(jy - r.y, -p.reach_y), p.reach_y), dx = min(max(jx - r.x, -p.reach_x), p.reach_x);
+    return __ldg(r.table + (dy + p.reach_y) * (2 * p.reach_x + 1) + dx + p.reach_x) * kLog2e;
+}
+
+// The score of key j times log2(e), from its product with the query.
+__device__ __forceinline__ float score2(const AttnDev &p, const Query &r, int j, float dot)
+{
+    float s = p.cap_out > 0.f ? p.cap_out * tanh_exp(dot * p.cap_in) : dot * p.scale;
+    if (p.bias == AJIB_BIAS_SLOPE) s -= r.slope * (float)abs(r.at - j);
+    if (p.bias == AJIB_BIAS_TABLE) {
+        const int jy = p.grid_w ? j / p.grid_w : 0;
+        s += table_bias(p, r, jy, j - jy * p.grid_w);
+    }
+    return s;
+}
+
+// One query of one head over keys [j0, j1), by one warp: the maximum m, the sum l and the
+// unnormalised outputs, o[e] for component lane + 32 e. qs: kMaxHeadDim floats of shared memory of
+// this warp. Keys and values that the query does not see are not read. A lane takes a key for the
+// scores, a component for the values.
+template <typename T>
+__device__ void attend_row(const AttnDev &p, int b, int h, int i, int qn, int kn, int j0, int j1, float *qs, float &m,
+                           float &l, float (&o)[8])
+{
+    const int lane = threadIdx.x & 31, g = h / p.group;
+    const T *q = (const T *)p.q + b * p.qb + i * p.qt + h * p.qh;
+    const T *k = (const T *)p.k + b * p.kb + g * p.kh, *v = (const T *)p.v + b * p.vb + g * p.vh;
+    for (int e = lane; e < p.d; e += 32) qs[e] = to_f(q[e]);
+    __syncwarp();
+    const Query r = query_of(p, b, h, i, qn, kn);
+    const int *docs = p.k_doc ? p.k_doc + (int64_t)(b % p.doc_rows) * p.lk : nullptr;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) o[e] = 0.f;
+    j1 = min(j1, kn);
+    for (int jt = j0; jt < j1; jt += 32) {
+        const int j = jt + lane;
+        const bool seen = j < j1 && in_reach(r, j) && (!docs || __ldg(docs + j) == r.doc);
+        const unsigned any = __ballot_sync(0xffffffffu, seen);
+        if (!any) continue;
+        float s = -INFINITY;
+        if (seen) {
+            const T *kj = k + j * p.kt;
+            float dot = 0.f;
+            for (int e = 0; e < p.d; e++) dot = fmaf(qs[e], to_f(kj[e]), dot);
+            s = score2(p, r, j, dot);
+        }
+        float top = s;
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, m);
+        const float base = top == -INFINITY ? 0.f : top, alpha = exp2_fast(m - base);
+        m = top;
+        const float e2 = seen ? exp2_fast(s - base) : 0.f;
+        float sum = e2;
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        l = l * alpha + sum;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] *= alpha;
+        for (int c = 0; c < 32; c++) {
+            if (!(any >> c & 1)) continue;
+            const float w = __shfl_sync(0xffffffffu, e2, c);
+            const T *vj = v + (jt + c) * p.vt;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (lane + 32 * e < p.d) o[e] = fmaf(w, to_f(vj[lane + 32 * e]), o[e]);
+        }
+    }
+    __syncwarp();
+}
+
+}  // namespace dev
+}  // namespace ajib

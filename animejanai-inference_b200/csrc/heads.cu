@@ -1,0 +1,298 @@
+/*
+ * heads.cu — rotary positions and the per-head norms of queries and keys (include/aji_b200.h,
+ * ajib_rotary_* and ajib_qk_launch).
+ *
+ * Both are one pass over the queries and keys: 2 bytes read and 2 written per element against a
+ * handful of fp32 operations, so memory bandwidth bounds them. A pair (x1, x2) at angle a becomes
+ * (x1 cos a - x2 sin a, x2 cos a + x1 sin a); the norm before it is one sum of squares over the
+ * head.
+ *
+ * Angles: position * frequency reaches 1e5 radians and more, where a float holds no useful
+ * fraction of a turn. Frequencies are kept as turns per position in 64-bit fixed point, so that the
+ * product wraps whole turns off by itself and the top 32 bits are the angle to 2^-32 of a turn
+ * (error below position * 2^-65 turns), for negative positions too.
+ */
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <new>
+
+#include "heads.h"
+
+struct ajib_rotary {
+    int dim = 0, layout = 0, axes = 1, grid_w = 0, n = 0;
+    double freq[ajib::kMaxHeadDim / 2];    // n = dim / 2 / axes angles per position
+    uint64_t turns[ajib::kMaxHeadDim / 2]; // the same, in 2^-64 turns
+    double amplitude = 1;
+};
+
+namespace ajib {
+namespace {
+
+constexpr int kQkThreads = 256;
+
+struct QkTensor {
+    const void *src;
+    void *dst;
+    int64_t sb, st, sh, ob, ot, oh;
+    const float *w;
+    int heads;
+};
+
+struct QkDev {
+    QkTensor t[2];
+    const int *pos, *len;
+    int64_t pos_sb, slots;
+    int pos0, tokens, d, rot, axes, grid_w, interleaved, norm, split;
+    float eps, amplitude;
+    uint64_t turns[kMaxHeadDim / 2];
+};
+
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// cos and sin of pair i (of npair) at a position, times the amplitude.
+__device__ __forceinline__ void pair_angle(const QkDev &p, int position, int i, float &c, float &s)
+{
+    int64_t at = position;
+    if (p.axes == 2) {
+        int row = position / p.grid_w;
+        if (position - row * p.grid_w < 0) row--;
+        const int per = p.rot >> 2;
+        if (i < per) {
+            at = row;
+        } else {
+            at = position - (int64_t)row * p.grid_w;
+            i -= per;
+        }
+    }
+    const uint64_t turn = (uint64_t)at * p.turns[i];
+    sincospif((float)(int)(turn >> 32) * 0x1p-31f, &s, &c);
+    c *= p.amplitude;
+    s *= p.amplitude;
+}
+
+__device__ __forceinline__ int position_of(const QkDev &p, int b, int t)
+{
+    return p.pos ? p.pos[b * p.pos_sb + t] : p.pos0 + t;
+}
+
+// A sum of squares that left the range of a float (bf16 heads near 1e19 and beyond, or tiny ones with
+// next to no eps) is taken again over values times this power of two. 1: the sum will do. (Below
+// 2^-80 against an eps of 2^-40 or more the sum does not matter.)
+__device__ __forceinline__ float rescale_of(const QkDev &p, float sum)
+{
+    return sum > 3.4e38f ? 0x1p-64f : sum < 0x1p-80f && p.eps < 0x1p-40f ? 0x1p64f : 1.f;
+}
+
+// What a head is multiplied by, from the sum of its squares times scale^2. Correctly rounded square
+// root and division: one each per head.
+__device__ __forceinline__ float norm_factor(const QkDev &p, float sum, float scale)
+{
+    if (p.norm == AJIB_NORM_RMS) return scale / sqrtf(sum / (float)p.d + p.eps * scale * scale);
+    const float n = sqrtf(sum) / scale;
+    return 1.f / (n < p.eps ? p.eps : n);  // not fmaxf, which drops a NaN
+}
+
+// One warp per head of one token, any d, alignment and rotary dim: lane l owns pairs l, l + 32, ...
+// and the components behind the turned ones. A lane reads the pair it writes, so in place is safe.
+template <typename T>
+__global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ QkDev p)
+{
+    const int64_t slot = ((int64_t)blockIdx.x * kQkThreads + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31;
+    if (slot >= p.slots) return;
+    const int heads = p.t[0].heads + p.t[1].heads;
+    const int64_t bt = slot / heads;
+    int h = (int)(slot - bt * heads);
+    const int b = (int)(bt / p.tokens), t = (int)(bt - (int64_t)b * p.tokens);
+    if (p.len && t >= p.len[b]) return;
+    const QkTensor &x = p.t[h >= p.t[0].heads];
+    if (h >= p.t[0].heads) h -= p.t[0].heads;
+    const T *src = (const T *)x.src + b * x.sb + t * x.st + h * x.sh;
+    T *dst = (T *)x.dst + b * x.ob + t * x.ot + h * x.oh;
+    float f = 1.f;
+    if (p.norm) {
+        float sum, scale = 1.f;
+        for (;;) {
+            sum = 0.f;
+            for (int i = lane; i < p.d; i += 32) {
+                const float v = to_f(src[i]) * scale;
+                sum += v * v;
+            }
+            for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+            if (scale != 1.f || (scale = rescale_of(p, sum)) == 1.f) break;
+        }
+        f = norm_factor(p, sum, scale);
+    }
+    const int npair = p.rot >> 1, position = p.rot ? position_of(p, b, t) : 0;
+    for (int i = lane; i < npair; i += 32) {
+        const int i1 = p.interleaved ? 2 * i : i, i2 = p.interleaved ? 2 * i + 1 : i + npair;
+        float x1 = to_f(src[i1]) * f, x2 = to_f(src[i2]) * f, c, s;
+        if (x.w) {
+            x1 *= x.w[i1];
+            x2 *= x.w[i2];
+        }
+        pair_angle(p, position, i, c, s);
+        dst[i1] = from_f<T>(x1 * c - x2 * s);
+        dst[i2] = from_f<T>(x2 * c + x1 * s);
+    }
+    for (int i = p.rot + lane; i < p.d; i += 32) {
+        float v = to_f(src[i]) * f;
+        if (x.w) v *= x.w[i];
+        dst[i] = from_f<T>(v);
+    }
+}
+
+template <typename T>
+cudaError_t run_qk(QkDev &p, const ajib_qk *op, int64_t rows, cudaStream_t s)
+{
+    const int64_t heads = p.t[0].heads + p.t[1].heads;
+    p.slots = rows * heads;
+    const int64_t blocks = (p.slots * 32 + kQkThreads - 1) / kQkThreads;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    k_qk_any<T><<<(unsigned)blocks, kQkThreads, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace ajib
+
+using namespace ajib;
+
+extern "C" int ajib_rotary_create(const ajib_rotary_params *p, ajib_rotary **out)
+{
+    if (!out) return AJIB_ERR_ARGS;
+    *out = nullptr;
+    if (!p || p->dim < 2 || p->dim > kMaxHeadDim || p->dim % 2) return AJIB_ERR_ARGS;
+    if (p->layout != AJIB_ROTARY_HALF && p->layout != AJIB_ROTARY_INTERLEAVED) return AJIB_ERR_ARGS;
+    if (p->axes != 1 && p->axes != 2) return AJIB_ERR_ARGS;
+    if (p->axes == 2 && (p->dim % 4 || p->grid_w < 1)) return AJIB_ERR_ARGS;
+    if (p->scaling < AJIB_ROTARY_PLAIN || p->scaling > AJIB_ROTARY_BANDS) return AJIB_ERR_ARGS;
+    if (!std::isfinite(p->amplitude) || p->amplitude < 0) return AJIB_ERR_ARGS;
+    const int n = p->dim / p->axes;
+    const double pi = 3.141592653589793238462643;
+    double f[kMaxHeadDim / 2], amp = 1;
+    if (p->freq) {
+        for (int i = 0; i < n / 2; i++) {
+            f[i] = p->freq[i];
+            if (!std::isfinite(f[i]) || f[i] < 0) return AJIB_ERR_ARGS;
+        }
+    } else {
+        double base = p->base;
+        if (!std::isfinite(base) || base <= 0) return AJIB_ERR_ARGS;
+        if (p->scaling != AJIB_ROTARY_PLAIN && (!std::isfinite(p->factor) || p->factor <= 0)) return AJIB_ERR_ARGS;
+        if (p->scaling == AJIB_ROTARY_BASE) {
+            if (n <= 2) return AJIB_ERR_ARGS;
+            base *= std::pow(p->factor, (double)n / (n - 2));
+        }
+        for (int i = 0; i < n / 2; i++) f[i] = std::pow(base, -2.0 * i / n);
+        if (p->scaling == AJIB_ROTARY_LINEAR)
+            for (int i = 0; i < n / 2; i++) f[i] /= p->factor;
+        if (p->scaling == AJIB_ROTARY_BANDS) {
+            const double fast = p->beta_fast == 0 ? 32 : p->beta_fast, slow = p->beta_slow == 0 ? 1 : p->beta_slow;
+            if (!std::isfinite(p->trained) || p->trained <= 0 || !std::isfinite(fast) || !std::isfinite(slow) || slow <= 0 || fast < slow ||
+                base <= 1)
+                return AJIB_ERR_ARGS;
+            // the pair whose frequency turns `beta` times over `trained` positions
+            auto pair = [&](double beta) { return n * std::log(p->trained / (beta * 2 * pi)) / (2 * std::log(base)); };
+            const double lo = std::fmax(std::floor(pair(fast)), 0), hi = std::fmin(std::ceil(pair(slow)), n - 1);
+            for (int i = 0; i < n / 2; i++) {
+                const double r = std::fmin(std::fmax((i - lo) / std::fmax(hi - lo, 0.001), 0), 1);
+                f[i] = f[i] / p->factor * r + f[i] * (1 - r);
+            }
+            amp = 0.1 * std::log(p->factor) + 1;
+        }
+        for (int i = 0; i < n / 2; i++)
+            if (!std::isfinite(f[i])) return AJIB_ERR_ARGS;
+    }
+    if (p->amplitude > 0) amp = p->amplitude;
+    ajib_rotary *r = new (std::nothrow) ajib_rotary;
+    if (!r) return AJIB_ERR_NO_MEM;
+    r->dim = p->dim;
+    r->layout = p->layout;
+    r->axes = p->axes;
+    r->grid_w = p->axes == 2 ? p->grid_w : 0;
+    r->n = n / 2;
+    r->amplitude = amp;
+    for (int i = 0; i < n / 2; i++) {
+        r->freq[i] = f[i];
+        const long double turn = fmodl((long double)f[i] / (2 * 3.14159265358979323846264338327950288L), 1.0L);
+        const long double fixed = rintl(ldexpl(turn, 64));
+        r->turns[i] = fixed >= ldexpl(1.0L, 64) ? 0 : (uint64_t)fixed;
+    }
+    *out = r;
+    return AJIB_OK;
+}
+
+extern "C" void ajib_rotary_release(ajib_rotary **r)
+{
+    if (!r || !*r) return;
+    delete *r;
+    *r = nullptr;
+}
+
+extern "C" int ajib_rotary_table(const ajib_rotary *r, double *freq, int n, double *amplitude)
+{
+    if (!r || n < 0) return AJIB_ERR_ARGS;
+    for (int i = 0; freq && i < n && i < r->n; i++) freq[i] = r->freq[i];
+    if (amplitude) *amplitude = r->amplitude;
+    return r->n;
+}
+
+extern "C" int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const ajib_heads *k, const ajib_heads *q_out,
+                              const ajib_heads *k_out, void *stream)
+{
+    if (!op || (op->dtype != AJIB_F16 && op->dtype != AJIB_BF16)) return AJIB_ERR_ARGS;
+    if (op->batch < 0 || op->tokens < 0 || op->hq < 1 || op->hk < 0 || op->d < 1 || op->d > kMaxHeadDim) return AJIB_ERR_ARGS;
+    if (op->batch > kMaxCount || op->tokens > kMaxCount || op->hq > kMaxCount || op->hk > kMaxCount) return AJIB_ERR_ARGS;
+    if (op->norm < AJIB_NORM_NONE || op->norm > AJIB_NORM_L2 || !(op->eps >= 0) || !std::isfinite(op->eps)) return AJIB_ERR_ARGS;
+    if (op->rotary && op->rotary->dim > op->d) return AJIB_ERR_ARGS;
+    if (op->pos && (((uintptr_t)op->pos & 3) || op->pos_sb < 0)) return AJIB_ERR_ARGS;
+    if (!op->pos && (int64_t)op->pos0 + op->tokens - 1 > 0x7fffffff) return AJIB_ERR_ARGS;
+    if (((uintptr_t)op->len & 3) || ((uintptr_t)op->wq & 3) || ((uintptr_t)op->wk & 3)) return AJIB_ERR_ARGS;
+    if (!op->batch || !op->tokens) return AJIB_OK;
+    const ajib_heads *in[2] = {q, k}, *out[2] = {q_out, k_out};
+    const int heads[2] = {op->hq, op->hk};
+    QkDev p{};
+    int width = 16;
+    for (int i = 0; i < 2 && heads[i]; i++) {
+        const int b = op->batch, t = op->tokens, h = heads[i];
+        if (!heads_ok(in[i], b, t, h, op->d) || !heads_ok(out[i], b, t, h, op->d)) return AJIB_ERR_ARGS;
+        if (!heads_distinct(out[i], b, t, h, op->d)) return AJIB_ERR_ARGS;
+        if (in[i]->p == out[i]->p && !heads_same(in[i], out[i])) return AJIB_ERR_ARGS;
+        if (i && (out[0]->p == out[1]->p || out[0]->p == in[1]->p || out[1]->p == in[0]->p)) return AJIB_ERR_ARGS;
+        p.t[i] = {in[i]->p, out[i]->p, in[i]->sb, in[i]->st, in[i]->sh, out[i]->sb, out[i]->st, out[i]->sh,
+                  op->norm ? (i ? op->wk : op->wq) : nullptr, h};
+        const int w1 = heads_width(in[i], b, t, h, op->d), w2 = heads_width(out[i], b, t, h, op->d);
+        width = width < w1 ? width : w1;
+        width = width < w2 ? width : w2;
+    }
+    p.pos = op->pos;
+    p.pos_sb = op->pos_sb;
+    p.pos0 = op->pos0;
+    p.len = op->len;
+    p.tokens = op->tokens;
+    p.d = op->d;
+    p.norm = op->norm;
+    p.eps = op->eps;
+    p.amplitude = 1.f;
+    if (const ajib_rotary *r = op->rotary) {
+        p.rot = r->dim;
+        p.axes = r->axes;
+        p.grid_w = r->grid_w;
+        p.interleaved = r->layout == AJIB_ROTARY_INTERLEAVED;
+        p.amplitude = (float)r->amplitude;
+        for (int i = 0; i < r->n; i++) p.turns[i] = r->turns[i];
+    }
+    const int64_t rows = (int64_t)op->batch * op->tokens;
+    const cudaError_t e = op->dtype == AJIB_F16 ? run_qk<__half>(p, op, rows, (cudaStream_t)stream)
+                                                : run_qk<__nv_bfloat16>(p, op, rows, (cudaStream_t)stream);
+    if (e == cudaErrorInvalidConfiguration) return AJIB_ERR_UNSUPPORTED;
+    return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
+}

@@ -330,6 +330,137 @@ AJIB_EXPORT int ajib_video_profile_read(aji_ctx *c, double *ms, int *counts, int
 /* device bytes held, launches per run */
 AJIB_EXPORT int ajib_exec_info(const ajib_exec *e, size_t *device_bytes, size_t *weight_bytes, int *launches);
 
+/* ---- attention operators ----
+ * The operators that mix tokens, beside the convolutions that mix pixels: rotary positions, the
+ * per-head norms of queries and keys, and attention, in fp16 or bf16 with fp32 arithmetic. The
+ * reference runs its image transformers' window attention inside those models' own code
+ * (src/native/tfm.h); here the operators stand alone, like the convolutions above. Inference only.
+ *
+ * A tensor of heads on the current device: component i of head h of token t of sequence b is the
+ * element at p + b * sb + t * st + h * sh + i (strides in elements, not negative; components are
+ * contiguous). A fused projection's queries, keys and values are three of these over one buffer, a
+ * cache is one whose st is its row. Inputs may repeat (stride 0); the elements of an output must be
+ * distinct (AJIB_ERR_ARGS otherwise). Pointers need the element's 2-byte alignment; with 16-byte
+ * aligned pointers and strides that are multiples of 8 the widest copies are used. */
+enum ajib_dtype { AJIB_F16 = 0, AJIB_BF16 = 1 };
+typedef struct ajib_heads {
+    void *p;
+    int64_t sb, st, sh;
+} ajib_heads;
+
+/* Rotary positions: which components turn, and by what angle per position.
+ * dim: how many leading components of a head turn, even, 2..256 (the others pass); they form
+ * dim / 2 pairs, (i, i + dim / 2) for AJIB_ROTARY_HALF or (2i, 2i + 1) for AJIB_ROTARY_INTERLEAVED.
+ * axes 1: pair i turns by position * f_i. axes 2 (tokens of a grid grid_w wide; dim a multiple of
+ * 4): the first half of the pairs turns by the row, position / grid_w rounded down, the second half
+ * by the column, each with the frequencies f_i of dim / 2 components.
+ * With n = dim / axes components, f_i = base^(-2 i / n), stretched for long contexts by `factor`:
+ *   AJIB_ROTARY_PLAIN   not at all
+ *   AJIB_ROTARY_LINEAR  f_i / factor
+ *   AJIB_ROTARY_BASE    base * factor^(n / (n - 2)) in place of base (n > 2)
+ *   AJIB_ROTARY_BANDS   frequencies that turn more than beta_fast times over `trained` positions
+ *                       stay, those that turn less than beta_slow times are divided by factor, a
+ *                       ramp over i between; beta 0: 32 and 1 (published as YaRN). The turned
+ *                       components are also scaled by 1 + 0.1 ln(factor) unless amplitude is given.
+ * amplitude: what the turned components are multiplied by; 0: 1, or the BANDS value.
+ * freq: NULL, or dim / 2 / axes angles per position (radians, finite, not negative) that replace
+ * base and scaling. */
+enum ajib_rotary_layout { AJIB_ROTARY_HALF = 0, AJIB_ROTARY_INTERLEAVED = 1 };
+enum ajib_rotary_scaling { AJIB_ROTARY_PLAIN = 0, AJIB_ROTARY_LINEAR = 1, AJIB_ROTARY_BASE = 2, AJIB_ROTARY_BANDS = 3 };
+typedef struct ajib_rotary_params {
+    int dim, layout, axes, grid_w, scaling;
+    double base, factor, trained, beta_fast, beta_slow, amplitude;
+    const double *freq;
+} ajib_rotary_params;
+typedef struct ajib_rotary ajib_rotary;
+/* The table lives on the host and travels with each launch: usable on every device, no device
+ * memory. AJIB_ERR_ARGS for parameters outside the ranges above. */
+AJIB_EXPORT int ajib_rotary_create(const ajib_rotary_params *p, ajib_rotary **out);
+AJIB_EXPORT void ajib_rotary_release(ajib_rotary **r);
+/* The frequencies (dim / 2 / axes of them; up to n are copied) and the amplitude; returns their
+ * number, or AJIB_ERR_ARGS. */
+AJIB_EXPORT int ajib_rotary_table(const ajib_rotary *r, double *freq, int n, double *amplitude);
+
+/* Norm and / or rotation of queries and keys, one kernel that reads and writes each once:
+ *   AJIB_NORM_RMS  x / sqrt(mean(x^2) + eps) * w     AJIB_NORM_L2  x / max(|x|, eps) * w
+ * over the d components of each head (w: wq for queries, wk for keys, d floats on the device; NULL:
+ * ones), then the rotation (rotary NULL: none), in fp32, rounded once. pos: NULL (token t stands at
+ * pos0 + t), or the int32 positions of batch x tokens, pos_sb elements from one sequence to the next
+ * (0: one row for all). len: NULL, or how many tokens of each sequence there are (int32, on the
+ * device; taken as 0..tokens): tokens behind are neither read nor written. d is 1..256. */
+enum ajib_norm { AJIB_NORM_NONE = 0, AJIB_NORM_RMS = 1, AJIB_NORM_L2 = 2 };
+typedef struct ajib_qk {
+    int dtype; /* enum ajib_dtype */
+    int batch, tokens, hq, hk, d; /* hk 0: queries alone */
+    const ajib_rotary *rotary;
+    int norm; /* enum ajib_norm */
+    float eps;
+    const float *wq, *wk;
+    const int32_t *pos;
+    int64_t pos_sb;
+    int pos0;
+    const int32_t *len;
+} ajib_qk;
+/* q -> q_out, k -> k_out (k and k_out are not looked at with hk 0). An output may be its own input
+ * (same pointer and strides); otherwise outputs overlap no input. k_out may be the rows of a cache.
+ * Batch or tokens of 0 do nothing. */
+AJIB_EXPORT int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const ajib_heads *k, const ajib_heads *q_out,
+                               const ajib_heads *k_out, void *stream);
+
+/* Attention of queries q over keys k and values v, softmax over the keys each query sees:
+ *   s = scale * q . k;  s = cap * tanh(s / cap) (cap > 0);  s += bias;  out = softmax(s) v
+ * Query head h reads key and value head h / (hq / hk) (hq a multiple of hk). Scores, softmax and
+ * sums are fp32; the probabilities are rounded to the type of v before their product with v.
+ *
+ * Where queries stand: key j of a sequence stands at j; query i stands at i, or with align_end at
+ * i + (keys - queries) of its sequence, so that the last query stands at the last key (new tokens
+ * over a cache). q_len, k_len: NULL, or how many queries and keys of each sequence there are
+ * (int32 [batch] on the device, taken as 0..lq and 0..lk). Queries behind are not written; keys
+ * and values behind are not looked at, whatever they hold.
+ *
+ * What query i at place p sees: key j < k_len where
+ *   - q_doc[i] == k_doc[j] and both are >= 0, if documents are given (int32 [doc_rows][lq] and
+ *     [doc_rows][lk], sequence b reads row b % doc_rows; a window mask's region ids, packed
+ *     sequences; negative: padding), and
+ *   - j < prefix of the sequence (int32 [batch], NULL: none), or else
+ *   - j <= p if causal, p - j <= left if left >= 0, and j - p <= right if right >= 0.
+ * A query that sees nothing gets zeros. What keys and values hold that a query does not see
+ * (infinities and NaN too) does not reach it.
+ *
+ * Bias, fp32 on the device: AJIB_BIAS_SLOPE adds -bias_data[h] * |p - j| (hq slopes);
+ * AJIB_BIAS_TABLE adds a table's entry for the distance of the key from the query, clamped to the
+ * table's reach: bias_data is [hq][2 reach_y + 1][2 reach_x + 1]. With grid_w 0 (reach_y 0) the
+ * distance is j - p; with grid_w > 0 places are (place / grid_w, place % grid_w) of a grid and the
+ * distances are those of rows and columns (window attention's relative positions; not with
+ * align_end).
+ *
+ * d is 1..256; lq and lk are up to 2^29 each (documents: lk up to 2^22). Zero batch or lq do
+ * nothing; with lk 0 every query gets zeros. Outputs overlap no input. */
+enum ajib_bias { AJIB_BIAS_NONE = 0, AJIB_BIAS_SLOPE = 1, AJIB_BIAS_TABLE = 2 };
+typedef struct ajib_attn {
+    int dtype; /* enum ajib_dtype */
+    int batch, lq, lk, hq, hk, d;
+    float scale, cap;
+    int causal, left, right; /* -1: no limit */
+    int align_end;
+    const int32_t *q_len, *k_len, *prefix;
+    const int32_t *q_doc, *k_doc;
+    int doc_rows;
+    int bias; /* enum ajib_bias */
+    const float *bias_data;
+    int grid_w, reach_y, reach_x;
+} ajib_attn;
+/* Bytes of device memory a launch of op needs on the current device (0 for most; few queries over
+ * many keys are split over the keys and joined through it), or 0 for an op that a launch refuses.
+ * 16-byte aligned; its contents need not be kept. Launches that may run at the same time, captured
+ * graphs' included, need one each. */
+AJIB_EXPORT size_t ajib_attention_workspace(const ajib_attn *op);
+/* AJIB_ERR_ARGS: arguments outside the above, or a workspace that is too small. Nothing is
+ * allocated; the call can be captured into a graph. */
+AJIB_EXPORT int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, const ajib_heads *k,
+                                      const ajib_heads *v, const ajib_heads *out, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+
 /* Reads and optionally clears the current device's kernel status word: 0, or the code of the
  * first pipeline wait that timed out in a kernel of this library. There is one word per device,
  * shared by every context and executor on it: a code may come from another context's kernels,
