@@ -4,46 +4,96 @@
  */
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
-#include "attention.cuh"
+#include "attention_mma.cuh"
 #include "heads.h"
 
 namespace ajib {
+
+int sm_count();  // conv.cu
+
 namespace {
 
 using namespace dev;
 
-constexpr int kRowWarps = 8;
+constexpr int kSplitTiles = 4;   // at least this many key tiles a split
+constexpr int kMaxSplits = 64;
 
-// One warp per query of a head: any d, alignment and stride.
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) k_attn_rows(const __grid_constant__ AttnDev p, int64_t rows)
+// How an op runs, from its sizes alone (the workspace must be known before the launch).
+struct Choice {
+    bool keys = false;  // few queries: the warps share the keys out
+    int row_tiles = 0, nsplit = 1;
+    int64_t rows = 0, blocks = 0;  // of a (sequence, key head); of the grid
+    size_t space = 0;
+};
+
+// Few queries (up to 64 rows a key head) share the keys out over warps, and over blocks until there
+// are two blocks an SM or a split has only kSplitTiles tiles.
+bool choose(const ajib_attn *op, Choice &c)
 {
-    __shared__ float qs[kRowWarps][kMaxHeadDim];
-    const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const int64_t bh = row / p.lq;
-    const int i = (int)(row - bh * p.lq), b = (int)(bh / p.hq), h = (int)(bh - (int64_t)b * p.hq);
-    const int qn = q_count(p, b), kn = k_count(p, b);
-    if (i >= qn) return;
-    float m, l, o[8];
-    attend_row<T>(p, b, h, i, qn, kn, 0, kn, qs[threadIdx.x >> 5], m, l, o);
-    T *out = (T *)p.out + b * p.ob + i * p.ot + h * p.oh;
-    const float f = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int c = (threadIdx.x & 31) + 32 * e;
-        if (c < p.d) out[c] = from_f<T>(l == 0.f ? 0.f : o[e] * f);
+    const int64_t group = op->hq / op->hk;
+    c.rows = op->lq * group;
+    if (c.rows > 1 << 30) return false;
+    c.keys = c.rows <= 64;
+    const int bm = c.keys ? 16 : 64;
+    c.row_tiles = (int)((c.rows + bm - 1) / bm);
+    const int64_t base = (int64_t)op->batch * op->hk;
+    c.blocks = base * c.row_tiles;
+    if (c.blocks > 0x7fffffff) return false;
+    if (c.keys && c.blocks) {
+        const int tiles = (op->lk + kMmaKeys - 1) / kMmaKeys;
+        const int64_t want = (2 * sm_count() + c.blocks - 1) / c.blocks;
+        c.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, tiles / kSplitTiles), kMaxSplits));
+        if (c.nsplit > 1) {
+            c.blocks *= c.nsplit;
+            const int64_t slots = base * c.rows * c.nsplit;
+            c.space = (size_t)slots * (8 + (size_t)op->d * 4);
+        }
     }
+    return c.blocks <= 0x7fffffff;
+}
+
+template <typename K>
+cudaError_t allow_smem(K kernel, int smem, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return cudaErrorInvalidDevice;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load() & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
+}
+
+constexpr int kMaxSmem = 227 * 1024;
+
+template <typename T, int DP, bool KEYS>
+cudaError_t run_mma(const MmaDev &p, const Choice &c, cudaStream_t s)
+{
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(k_attn_mma<T, DP, KEYS>, kMaxSmem, done);
+    if (e != cudaSuccess) return e;
+    k_attn_mma<T, DP, KEYS><<<(unsigned)c.blocks, kMmaThreads, MmaCfg<DP, KEYS>::smem(p.a), s>>>(p);
+    return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t run(const AttnDev &p, cudaStream_t s)
+cudaError_t run(const MmaDev &p, const Choice &c, cudaStream_t s)
 {
-    const int64_t rows = (int64_t)p.batch * p.hq * p.lq, blocks = (rows + kRowWarps - 1) / kRowWarps;
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    k_attn_rows<T><<<(unsigned)blocks, kRowWarps * 32, 0, s>>>(p, rows);
+    const int d = p.a.d;
+    cudaError_t e;
+    if (c.keys)
+        e = d <= 32 ? run_mma<T, 32, true>(p, c, s) : d <= 64 ? run_mma<T, 64, true>(p, c, s)
+            : d <= 128 ? run_mma<T, 128, true>(p, c, s) : run_mma<T, 256, true>(p, c, s);
+    else
+        e = d <= 32 ? run_mma<T, 32, false>(p, c, s) : d <= 64 ? run_mma<T, 64, false>(p, c, s)
+            : d <= 128 ? run_mma<T, 128, false>(p, c, s) : run_mma<T, 256, false>(p, c, s);
+    if (e != cudaSuccess || c.nsplit == 1) return e;
+    const int64_t rows = (int64_t)p.a.batch * p.a.hk * p.rows;
+    k_attn_join<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -81,8 +131,8 @@ using namespace ajib;
 
 extern "C" size_t ajib_attention_workspace(const ajib_attn *op)
 {
-    if (!check(op)) return 0;
-    return 0;
+    Choice c;
+    return check(op) && choose(op, c) ? c.space : 0;
 }
 
 extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, const ajib_heads *k, const ajib_heads *v,
@@ -97,7 +147,11 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         if (!heads_ok(k, b, op->lk, op->hk, d) || !heads_ok(v, b, op->lk, op->hk, d)) return AJIB_ERR_ARGS;
         if (out->p == k->p || out->p == v->p) return AJIB_ERR_ARGS;
     }
-    AttnDev p{};
+    Choice c;
+    if (!choose(op, c)) return AJIB_ERR_UNSUPPORTED;
+    if (c.space && (!workspace || workspace_bytes < c.space || ((uintptr_t)workspace & 15))) return AJIB_ERR_ARGS;
+    MmaDev m{};
+    AttnDev &p = m.a;
     p.q = q->p;
     p.out = out->p;
     p.qb = q->sb, p.qt = q->st, p.qh = q->sh;
@@ -136,8 +190,23 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
     p.reach_y = op->reach_y;
     p.reach_x = op->reach_x;
     p.masked = p.left != far || p.right != far || p.q_doc;
-    const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(p, (cudaStream_t)stream)
-                                                : run<__nv_bfloat16>(p, (cudaStream_t)stream);
-    if (e == cudaErrorInvalidConfiguration) return AJIB_ERR_UNSUPPORTED;
+    m.rows = (int)c.rows;
+    m.row_tiles = c.row_tiles;
+    m.nsplit = c.nsplit;
+    m.wq = heads_width(q, b, op->lq, op->hq, d);
+    m.wo = heads_width(out, b, op->lq, op->hq, d);
+    m.wkv = op->lk ? std::min(heads_width(k, b, op->lk, op->hk, d), heads_width(v, b, op->lk, op->hk, d)) : 16;
+    const int64_t slots = (int64_t)b * op->hk * c.rows * c.nsplit;
+    m.part_ml = (float2 *)workspace;
+    m.part = (float *)workspace + 2 * slots;
+    m.bias_form = op->bias == AJIB_BIAS_SLOPE ? kBiasSlope : kBiasNone;
+    if (op->bias == AJIB_BIAS_TABLE) {
+        // a table that reaches every distance of the grid is read without clamps
+        const bool reached = op->grid_w && op->reach_x >= op->grid_w - 1 &&
+                             op->reach_y >= (std::max(op->lq, op->lk) - 1) / op->grid_w;
+        m.bias_form = !op->grid_w ? kBiasLine : reached ? kBiasGridDirect : kBiasGrid;
+    }
+    const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(m, c, (cudaStream_t)stream)
+                                                : run<__nv_bfloat16>(m, c, (cudaStream_t)stream);
     return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
 }
