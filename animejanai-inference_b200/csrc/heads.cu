@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -46,7 +47,7 @@ struct QkDev {
     const int *pos, *len;
     int64_t pos_sb, slots;
     int pos0, tokens, d, rot, axes, grid_w, interleaved, norm, split;
-    float eps, amplitude;
+    float eps, amplitude, inv_d, inv_eps;
     uint64_t turns[kMaxHeadDim / 2];
 };
 
@@ -90,13 +91,12 @@ __device__ __forceinline__ float rescale_of(const QkDev &p, float sum)
     return sum > 3.4e38f ? 0x1p-64f : sum < 0x1p-80f && p.eps < 0x1p-40f ? 0x1p64f : 1.f;
 }
 
-// What a head is multiplied by, from the sum of its squares times scale^2. Correctly rounded square
-// root and division: one each per head.
+// What a head is multiplied by, from the sum of its squares times scale^2 (rsqrt: 2 ulp).
 __device__ __forceinline__ float norm_factor(const QkDev &p, float sum, float scale)
 {
-    if (p.norm == AJIB_NORM_RMS) return scale / sqrtf(sum / (float)p.d + p.eps * scale * scale);
-    const float n = sqrtf(sum) / scale;
-    return 1.f / (n < p.eps ? p.eps : n);  // not fmaxf, which drops a NaN
+    if (p.norm == AJIB_NORM_RMS) return scale * rsqrtf(sum * p.inv_d + p.eps * scale * scale);
+    const float f = scale * rsqrtf(sum);
+    return f > p.inv_eps ? p.inv_eps : f;  // not fminf, which drops a NaN
 }
 
 // One warp per head of one token, any d, alignment and rotary dim: lane l owns pairs l, l + 32, ...
@@ -149,10 +149,187 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ Q
     }
 }
 
-template <typename T>
-cudaError_t run_qk(QkDev &p, const ajib_qk *op, int64_t rows, cudaStream_t s)
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+template <> struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ float2 unpack(uint32_t v)
+    {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+
+// d and the turned components multiples of 16, every row 16-byte aligned: a lane holds two chunks of 8
+// components of a head (16-byte loads, neighbouring lanes on neighbouring chunks), GP lanes (a power of
+// two, d / 16 of them at work) a head. HALF: chunk g of the turned components' first half and of their
+// second, so that pairs meet in a lane; otherwise chunk g of a half of what there is. A lane computes
+// its 8 angles once and walks the heads of its token, `split` groups to a token so that small batches
+// fill the machine too. U heads are in flight at a time: DRAM latency times bandwidth is some 45 KB an
+// SM, four blocks of 256 lanes with 64 bytes each hold 64 KB.
+template <typename T, int GP, bool NORM, bool TURN>
+__global__ void __launch_bounds__(kQkThreads, NORM && TURN ? 3 : 4) k_qk_vec(const __grid_constant__ QkDev p)
 {
-    const int64_t heads = p.t[0].heads + p.t[1].heads;
+    const uint32_t slot = blockIdx.x * (kQkThreads / GP) + threadIdx.x / GP;  // (below 2^32: run_qk)
+    const int g = threadIdx.x % GP;
+    const bool there = slot < (uint32_t)p.slots;
+    const uint32_t at = there ? slot : (uint32_t)p.slots - 1;
+    const uint32_t bt = at / p.split;
+    const int h0 = (int)(at - bt * p.split);
+    const int b = (int)(bt / p.tokens), t = (int)(bt - (uint32_t)b * p.tokens);
+    // lanes of a warp stay together for the sums: what a lane has no part in, it neither reads nor writes
+    const bool live = there && g * 16 < p.d && !(p.len && t >= p.len[b]);
+    const bool apart = TURN && !p.interleaved;
+    int c1 = 8 * g, c2 = (p.d >> 1) + 8 * g;
+    if (apart) {
+        const int turned = p.rot >> 4, rest = (p.d - p.rot) >> 1;  // lanes at work on each part
+        c1 = g < turned ? 8 * g : p.rot + 8 * (g - turned);
+        c2 = c1 + (g < turned ? p.rot >> 1 : rest);
+    }
+    float c[8], s[8];
+    if (TURN) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = 1.f, s[i] = 0.f;
+        if (live && c1 < p.rot) {
+            const int position = position_of(p, b, t);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int pair = apart ? c1 + i : (i < 4 ? c1 >> 1 : (c2 >> 1) - 4) + i;
+                if (2 * pair < p.rot) pair_angle(p, position, pair, c[i], s[i]);
+            }
+        }
+    }
+    const unsigned all = ((1u << GP) - 1) << (threadIdx.x % 32 / GP * GP);
+    int h = h0;
+    for (int part = 0; part < 2; part++) {
+        const QkTensor &q = p.t[part];
+        float w1[8], w2[8];
+        if (NORM) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w1[i] = live && q.w ? __ldg(q.w + c1 + i) : 1.f;
+                w2[i] = live && q.w ? __ldg(q.w + c2 + i) : 1.f;
+            }
+        }
+        const T *src = (const T *)q.src + b * q.sb + t * q.st + h * q.sh;
+        T *dst = (T *)q.dst + b * q.ob + t * q.ot + h * q.oh;
+        const int64_t step = p.split * q.sh, out_step = p.split * q.oh;
+        constexpr int U = 2;  // heads in flight
+        for (; h < q.heads; h += U * p.split) {  // (uniform over the lanes of a head)
+            uint4 x[U][2];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
+                if (live && h + u * p.split < q.heads) {
+                    x[u][0] = *reinterpret_cast<const uint4 *>(src + u * step + c1);
+                    x[u][1] = *reinterpret_cast<const uint4 *>(src + u * step + c2);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float a[8], e[8];
+                const uint32_t *xa = &x[u][0].x, *xe = &x[u][1].x;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 fa = Pair<T>::unpack(xa[i]), fe = Pair<T>::unpack(xe[i]);
+                    a[2 * i] = fa.x, a[2 * i + 1] = fa.y;
+                    e[2 * i] = fe.x, e[2 * i + 1] = fe.y;
+                }
+                if (NORM) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sum = fmaf(a[i], a[i], fmaf(e[i], e[i], sum));
+#pragma unroll
+                    for (int m = GP / 2; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
+                    const float scale = rescale_of(p, sum);
+                    if (scale != 1.f) {  // (every lane of the head agrees)
+                        sum = 0.f;
+                        for (int i = 0; i < 8; i++)
+                            sum += (a[i] * scale) * (a[i] * scale) + (e[i] * scale) * (e[i] * scale);
+                        for (int m = GP / 2; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
+                    }
+                    const float f = norm_factor(p, sum, scale);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        a[i] = a[i] * f * w1[i];
+                        e[i] = e[i] * f * w2[i];
+                    }
+                }
+                if (TURN) {  // (what does not turn has angle 0)
+                    if (apart) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float x1 = a[i], x2 = e[i];
+                            a[i] = x1 * c[i] - x2 * s[i];
+                            e[i] = x2 * c[i] + x1 * s[i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float x1 = a[2 * i], x2 = a[2 * i + 1], y1 = e[2 * i], y2 = e[2 * i + 1];
+                            a[2 * i] = x1 * c[i] - x2 * s[i];
+                            a[2 * i + 1] = x2 * c[i] + x1 * s[i];
+                            e[2 * i] = y1 * c[4 + i] - y2 * s[4 + i];
+                            e[2 * i + 1] = y2 * c[4 + i] + y1 * s[4 + i];
+                        }
+                    }
+                }
+                if (live && h + u * p.split < q.heads) {
+                    *reinterpret_cast<uint4 *>(dst + u * out_step + c1) =
+                        make_uint4(Pair<T>::pack(a[0], a[1]), Pair<T>::pack(a[2], a[3]), Pair<T>::pack(a[4], a[5]),
+                                   Pair<T>::pack(a[6], a[7]));
+                    *reinterpret_cast<uint4 *>(dst + u * out_step + c2) =
+                        make_uint4(Pair<T>::pack(e[0], e[1]), Pair<T>::pack(e[2], e[3]), Pair<T>::pack(e[4], e[5]),
+                                   Pair<T>::pack(e[6], e[7]));
+                }
+            }
+            src += U * step;
+            dst += U * out_step;
+        }
+        // the same walk goes on in the keys: the first place at or behind the last query head
+        h = h0 >= q.heads ? h0 - q.heads : (p.split - (q.heads - h0) % p.split) % p.split;
+    }
+}
+
+template <typename T, int GP>
+cudaError_t run_vec(const QkDev &p, cudaStream_t s)
+{
+    const int64_t blocks = (p.slots * GP + kQkThreads - 1) / kQkThreads;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const unsigned n = (unsigned)blocks;
+    if (p.norm && p.rot)
+        k_qk_vec<T, GP, true, true><<<n, kQkThreads, 0, s>>>(p);
+    else if (p.norm)
+        k_qk_vec<T, GP, true, false><<<n, kQkThreads, 0, s>>>(p);
+    else
+        k_qk_vec<T, GP, false, true><<<n, kQkThreads, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_qk(QkDev &p, int width, int64_t rows, cudaStream_t s)
+{
+    const int heads = p.t[0].heads + p.t[1].heads;
+    if (width == 16 && p.d % 16 == 0 && p.rot % 16 == 0 && (p.norm || p.rot)) {
+        const int g = p.d / 16;
+        // groups of lanes to a token: one does all its heads once that gives every SM 2048 lanes
+        const int64_t lanes = rows * g, want = 148 * 2048;
+        p.split = (int)std::min<int64_t>(heads, std::max<int64_t>(1, (want + lanes - 1) / lanes));
+        p.slots = rows * p.split;
+        if (p.slots < 1ll << 31)
+            return g == 1 ? run_vec<T, 1>(p, s) : g == 2 ? run_vec<T, 2>(p, s) : g <= 4 ? run_vec<T, 4>(p, s)
+                   : g <= 8 ? run_vec<T, 8>(p, s) : run_vec<T, 16>(p, s);
+    }
     p.slots = rows * heads;
     const int64_t blocks = (p.slots * 32 + kQkThreads - 1) / kQkThreads;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
@@ -281,6 +458,8 @@ extern "C" int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const ajib
     p.d = op->d;
     p.norm = op->norm;
     p.eps = op->eps;
+    p.inv_d = 1.f / op->d;
+    p.inv_eps = 1.f / op->eps;  // (eps 0: infinity)
     p.amplitude = 1.f;
     if (const ajib_rotary *r = op->rotary) {
         p.rot = r->dim;
@@ -291,8 +470,8 @@ extern "C" int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const ajib
         for (int i = 0; i < r->n; i++) p.turns[i] = r->turns[i];
     }
     const int64_t rows = (int64_t)op->batch * op->tokens;
-    const cudaError_t e = op->dtype == AJIB_F16 ? run_qk<__half>(p, op, rows, (cudaStream_t)stream)
-                                                : run_qk<__nv_bfloat16>(p, op, rows, (cudaStream_t)stream);
+    const cudaError_t e = op->dtype == AJIB_F16 ? run_qk<__half>(p, width, rows, (cudaStream_t)stream)
+                                                : run_qk<__nv_bfloat16>(p, width, rows, (cudaStream_t)stream);
     if (e == cudaErrorInvalidConfiguration) return AJIB_ERR_UNSUPPORTED;
     return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
 }
