@@ -9,11 +9,14 @@
 #include <cmath>
 
 #include "attention_mma.cuh"
+#include "attention_tc.cuh"
+#include "cuctx.h"
 #include "heads.h"
 
 namespace ajib {
 
 int sm_count();  // conv.cu
+int *attn_status_word();
 
 namespace {
 
@@ -21,10 +24,12 @@ using namespace dev;
 
 constexpr int kSplitTiles = 4;   // at least this many key tiles a split
 constexpr int kMaxSplits = 64;
+constexpr int kTcQueries = 256;  // tcgen05 from here on (queries and keys)
 
 // How an op runs, from its sizes alone (the workspace must be known before the launch).
 struct Choice {
     bool keys = false;  // few queries: the warps share the keys out
+    bool tc = false;    // long prompts, if the tensors' layout allows: 256 queries a block on tcgen05
     int row_tiles = 0, nsplit = 1;
     int64_t rows = 0, blocks = 0;  // of a (sequence, key head); of the grid
     size_t space = 0;
@@ -38,6 +43,9 @@ bool choose(const ajib_attn *op, Choice &c)
     c.rows = op->lq * group;
     if (c.rows > 1 << 30) return false;
     c.keys = c.rows <= 64;
+    c.tc = !c.keys && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d > 32 && op->d <= 128 && op->d % 8 == 0 &&
+           !(op->bias == AJIB_BIAS_TABLE && op->grid_w) &&
+           (int64_t)op->batch * op->hq * ((op->lq + 255) / 256) <= 0x7fffffff;
     const int bm = c.keys ? 16 : 64;
     c.row_tiles = (int)((c.rows + bm - 1) / bm);
     const int64_t base = (int64_t)op->batch * op->hk;
@@ -97,6 +105,46 @@ cudaError_t run(const MmaDev &p, const Choice &c, cudaStream_t s)
     return cudaGetLastError();
 }
 
+// A tensor map of 128-token tiles of 64 components of one head (128-byte swizzle; zeros outside).
+// False if the layout does not allow one (16-byte aligned, no repeated dimension).
+bool map_of(CUtensorMap *m, const ajib_heads *x, int batch, int tokens, int heads, int d, int dtype)
+{
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? (Encode)fn : nullptr;
+    }();
+    if (!encode || heads_width(x, batch, tokens, heads, d) != 16) return false;
+    const int n[3] = {tokens, heads, batch};
+    const int64_t st[3] = {x->st, x->sh, x->sb};
+    cuuint64_t dims[4] = {(cuuint64_t)d, 0, 0, 0}, strides[3];
+    for (int i = 0; i < 3; i++) {
+        if (n[i] > 1 && (st[i] <= 0 || st[i] >= 1ll << 38)) return false;
+        dims[i + 1] = (cuuint64_t)n[i];
+        strides[i] = n[i] > 1 ? (cuuint64_t)st[i] * 2 : 16;  // (never used)
+    }
+    const cuuint32_t box[4] = {64, 128, 1, 1}, one[4] = {1, 1, 1, 1};
+    return encode(m, dtype == AJIB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x->p, dims,
+                  strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP>
+cudaError_t run_tc(const TcDev &p, const CUtensorMap (&m)[3], cudaStream_t s)
+{
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(k_attn_tc<T, DP>, kMaxSmem, done);
+    if (e != cudaSuccess) return e;
+    const int64_t blocks = (int64_t)p.a.batch * p.a.hq * p.tiles;
+    k_attn_tc<T, DP><<<(unsigned)blocks, kTcThreads, TcCfg<DP>::smem(p.a), s>>>(p, m[0], m[1], m[2]);
+    return cudaGetLastError();
+}
+
 bool misaligned4(const void *p) { return ((uintptr_t)p & 3) != 0; }
 
 // Everything but the tensors.
@@ -126,6 +174,16 @@ bool check(const ajib_attn *op)
 
 }  // namespace
 }  // namespace ajib
+
+// The attention kernels' status word: of this library's image on the device, so that a first launch
+// needs no allocation and can be captured. ajib_kernel_status reads it with the convolutions'.
+__device__ int g_attn_status;
+
+int *ajib::attn_status_word()
+{
+    void *p = nullptr;
+    return cudaGetSymbolAddress(&p, g_attn_status) == cudaSuccess ? (int *)p : nullptr;
+}
 
 using namespace ajib;
 
@@ -205,6 +263,23 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         const bool reached = op->grid_w && op->reach_x >= op->grid_w - 1 &&
                              op->reach_y >= (std::max(op->lq, op->lk) - 1) / op->grid_w;
         m.bias_form = !op->grid_w ? kBiasLine : reached ? kBiasGridDirect : kBiasGrid;
+    }
+    CUtensorMap maps[3];
+    if (c.tc && map_of(&maps[0], q, b, op->lq, op->hq, d, op->dtype) && map_of(&maps[1], k, b, op->lk, op->hk, d, op->dtype) &&
+        map_of(&maps[2], v, b, op->lk, op->hk, d, op->dtype)) {
+        TcDev t{};
+        t.a = p;
+        t.tiles = (op->lq + 255) / 256;
+        t.bias_form = m.bias_form;
+        t.scaled = op->cap > 0 || op->bias != AJIB_BIAS_NONE || !(op->scale > 0);
+        t.wo = m.wo;
+        t.err = attn_status_word();
+        if (!t.err) return AJIB_ERR_CUDA;
+        const bool f16 = op->dtype == AJIB_F16;
+        const cudaStream_t s = (cudaStream_t)stream;
+        const cudaError_t e = d <= 64 ? (f16 ? run_tc<__half, 64>(t, maps, s) : run_tc<__nv_bfloat16, 64>(t, maps, s))
+                                      : (f16 ? run_tc<__half, 128>(t, maps, s) : run_tc<__nv_bfloat16, 128>(t, maps, s));
+        return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
     }
     const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(m, c, (cudaStream_t)stream)
                                                 : run<__nv_bfloat16>(m, c, (cudaStream_t)stream);

@@ -88,11 +88,11 @@ __device__ __forceinline__ Query query_of(const AttnDev &p, int b, int h, int i,
     r.at = i + (p.align_end ? kn - qn : 0);
     r.lo = p.left == INT_MAX / 2 ? INT_MIN : r.at - p.left;
     r.hi = p.right == INT_MAX / 2 ? INT_MAX : r.at + p.right;
-    r.pre = p.prefix ? __ldg(p.prefix + b) : 0;
+    r.pre = p.prefix ? max(__ldg(p.prefix + b), 0) : 0;
     r.doc = INT_MIN;
     if (p.q_doc) {
         r.doc = i < p.lq ? __ldg(p.q_doc + (int64_t)(b % p.doc_rows) * p.lq + i) : -1;
-        if (r.doc < 0) r.lo = INT_MAX, r.hi = r.pre = INT_MIN;  // padding sees nothing
+        if (r.doc < 0) r.lo = INT_MAX, r.hi = -1, r.pre = 0;  // padding sees nothing
     }
     r.y = 0;
     r.x = r.at;

@@ -37,6 +37,8 @@ struct ajib_weights {
 
 namespace ajib {
 
+int *attn_status_word();  // attention.cu
+
 int pad_k(int cin) { return cin <= 16 ? 16 : (cin + 15) / 16 * 16; }
 // 3x3 outputs pad to 16, 32, 48 or 64 columns. 48 channels (SPAN, SPANF3) keep their width: a
 // row's stacked-tap MMA is then N = 144 rather than 192 (a quarter fewer tensor cycles), and the
@@ -597,12 +599,15 @@ extern "C" size_t ajib_feature_bytes(int H, int W, int C)
 
 extern "C" int ajib_kernel_status(int clear)
 {
-    int *w = status_word();
-    if (!w) return AJIB_ERR_CUDA;
-    int v = 0;
-    if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return AJIB_ERR_CUDA;
-    if (clear && v && cudaMemset(w, 0, sizeof(int)) != cudaSuccess) return AJIB_ERR_CUDA;
-    return v;
+    int first = 0;
+    for (int *w : {status_word(), attn_status_word()}) {
+        if (!w) return AJIB_ERR_CUDA;
+        int v = 0;
+        if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return AJIB_ERR_CUDA;
+        if (clear && v && cudaMemset(w, 0, sizeof(int)) != cudaSuccess) return AJIB_ERR_CUDA;
+        if (!first) first = v;
+    }
+    return first;
 }
 
 // ---- the model input packed into a strip-chunked map (the executor's head path) ----
