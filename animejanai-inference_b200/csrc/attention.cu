@@ -24,7 +24,7 @@ using namespace dev;
 
 constexpr int kSplitTiles = 4;   // at least this many key tiles a split
 constexpr int kMaxSplits = 64;
-constexpr int kTcQueries = 256;  // tcgen05 from here on (queries and keys)
+constexpr int kTcQueries = 192;  // tcgen05 from here on (queries and keys)
 
 // How an op runs, from its sizes alone (the workspace must be known before the launch).
 struct Choice {
@@ -35,6 +35,14 @@ struct Choice {
     size_t space = 0;
 };
 
+constexpr int kMaxSmem = 227 * 1024;
+
+// Whether the table of a grid reaches every distance on it: then it is read without clamps.
+bool grid_reached(const ajib_attn *op)
+{
+    return op->reach_x >= op->grid_w - 1 && op->reach_y >= (std::max(op->lq, op->lk) - 1) / op->grid_w;
+}
+
 // Few queries (up to 64 rows a key head) share the keys out over warps, and over blocks until there
 // are two blocks an SM or a split has only kSplitTiles tiles.
 bool choose(const ajib_attn *op, Choice &c)
@@ -43,9 +51,11 @@ bool choose(const ajib_attn *op, Choice &c)
     c.rows = op->lq * group;
     if (c.rows > 1 << 30) return false;
     c.keys = c.rows <= 64;
-    c.tc = !c.keys && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d > 32 && op->d <= 128 && op->d % 8 == 0 &&
-           !(op->bias == AJIB_BIAS_TABLE && op->grid_w) &&
-           (int64_t)op->batch * op->hq * ((op->lq + 255) / 256) <= 0x7fffffff;
+    if (!c.keys && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d <= 128 && op->d % 8 == 0) {
+        const bool grid = op->bias == AJIB_BIAS_TABLE && op->grid_w;
+        c.tc = (!grid || grid_reached(op)) && (int64_t)op->batch * op->hq * ((op->lq + 255) / 256) <= 0x7fffffff &&
+               (op->d <= 64 ? TcCfg<64>::smem(op) : TcCfg<128>::smem(op)) <= kMaxSmem;
+    }
     const int bm = c.keys ? 16 : 64;
     c.row_tiles = (int)((c.rows + bm - 1) / bm);
     const int64_t base = (int64_t)op->batch * op->hk;
@@ -75,8 +85,6 @@ cudaError_t allow_smem(K kernel, int smem, std::atomic<uint64_t> &done)
     if (e == cudaSuccess) done.fetch_or(bit);
     return e;
 }
-
-constexpr int kMaxSmem = 227 * 1024;
 
 template <typename T, int DP, bool KEYS>
 cudaError_t run_mma(const MmaDev &p, const Choice &c, cudaStream_t s)
@@ -135,13 +143,15 @@ bool map_of(CUtensorMap *m, const ajib_heads *x, int batch, int tokens, int head
 }
 
 template <typename T, int DP>
-cudaError_t run_tc(const TcDev &p, const CUtensorMap (&m)[3], cudaStream_t s)
+cudaError_t run_tc(TcDev &p, const ajib_attn *op, const CUtensorMap (&m)[3], cudaStream_t s)
 {
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(k_attn_tc<T, DP>, kMaxSmem, done);
     if (e != cudaSuccess) return e;
-    const int64_t blocks = (int64_t)p.a.batch * p.a.hq * p.tiles;
-    k_attn_tc<T, DP><<<(unsigned)blocks, kTcThreads, TcCfg<DP>::smem(p.a), s>>>(p, m[0], m[1], m[2]);
+    p.words = TcCfg<DP>::bit_words(op);
+    p.table_st = TcCfg<DP>::table_stride(op);
+    const unsigned blocks = (unsigned)std::min<int64_t>(p.items, sm_count());
+    k_attn_tc<T, DP><<<blocks, kTcThreads, (int)TcCfg<DP>::smem(op), s>>>(p, m[0], m[1], m[2]);
     return cudaGetLastError();
 }
 
@@ -259,10 +269,7 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
     m.part = (float *)workspace + 2 * slots;
     m.bias_form = op->bias == AJIB_BIAS_SLOPE ? kBiasSlope : kBiasNone;
     if (op->bias == AJIB_BIAS_TABLE) {
-        // a table that reaches every distance of the grid is read without clamps
-        const bool reached = op->grid_w && op->reach_x >= op->grid_w - 1 &&
-                             op->reach_y >= (std::max(op->lq, op->lk) - 1) / op->grid_w;
-        m.bias_form = !op->grid_w ? kBiasLine : reached ? kBiasGridDirect : kBiasGrid;
+        m.bias_form = !op->grid_w ? kBiasLine : grid_reached(op) ? kBiasGridDirect : kBiasGrid;
     }
     CUtensorMap maps[3];
     if (c.tc && map_of(&maps[0], q, b, op->lq, op->hq, d, op->dtype) && map_of(&maps[1], k, b, op->lk, op->hk, d, op->dtype) &&
@@ -270,15 +277,19 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         TcDev t{};
         t.a = p;
         t.tiles = (op->lq + 255) / 256;
+        t.items = (int64_t)b * op->hq * t.tiles;
         t.bias_form = m.bias_form;
+        t.head_major = m.bias_form == kBiasGridDirect;
         t.scaled = op->cap > 0 || op->bias != AJIB_BIAS_NONE || !(op->scale > 0);
-        t.wo = m.wo;
+        const uint64_t rows = (uint64_t)(uintptr_t)out->p | (uint64_t)d * 2 | (uint64_t)(b > 1 ? out->sb : 0) * 2 |
+                              (uint64_t)out->st * 2 | (uint64_t)(op->hq > 1 ? out->sh : 0) * 2;
+        t.wo = rows % 32 == 0 ? 32 : m.wo;
         t.err = attn_status_word();
         if (!t.err) return AJIB_ERR_CUDA;
         const bool f16 = op->dtype == AJIB_F16;
         const cudaStream_t s = (cudaStream_t)stream;
-        const cudaError_t e = d <= 64 ? (f16 ? run_tc<__half, 64>(t, maps, s) : run_tc<__nv_bfloat16, 64>(t, maps, s))
-                                      : (f16 ? run_tc<__half, 128>(t, maps, s) : run_tc<__nv_bfloat16, 128>(t, maps, s));
+        const cudaError_t e = d <= 64 ? (f16 ? run_tc<__half, 64>(t, op, maps, s) : run_tc<__nv_bfloat16, 64>(t, op, maps, s))
+                                      : (f16 ? run_tc<__half, 128>(t, op, maps, s) : run_tc<__nv_bfloat16, 128>(t, op, maps, s));
         return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
     }
     const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(m, c, (cudaStream_t)stream)

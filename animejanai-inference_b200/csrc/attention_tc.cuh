@@ -3,7 +3,7 @@
  *
  * A block takes 256 queries of one head as two tiles of 128 and walks the keys in tiles of 128.
  * Warps 0-3 and 4-7 do the softmax of one query tile each (a thread a row), warp 8 issues the TMA
- * copies, warp 9 the matrix products:
+ * copies, warp 9 the matrix products, warps 10 and 11 look up which key tiles hold which documents:
  *   S_q = Q_q K^T   (both from shared memory)       -> TMEM, 128 columns each
  *   O_q += P_q V    (P from TMEM, V from shared)    -> TMEM, DP columns each
  * P_q takes the columns of S_q: a thread holds its whole row of scores in registers before it writes
@@ -14,6 +14,9 @@
  * 2^8: the accumulators are rescaled rarely, and by the softmax threads themselves, at a time when
  * no product touches them. Probabilities are then up to 2^8 instead of 1, which costs neither fp16
  * nor bf16 any precision.
+ *
+ * Blocks stay and walk items of 256 queries: copies and products of the next item run while the
+ * softmax warps still write the last one out.
  *
  * What bounds it: per 256 x 128 scores the tensor pipe needs 32 * DP cycles (8192 flop a cycle)
  * and the exponentials 2048 (16 a cycle): even at DP 128, exponentials at 64.
@@ -32,10 +35,14 @@ constexpr int kTcThreads = 384, kTcKeys = 128;
 
 struct TcDev {
     AttnDev a;
-    int tiles;      // of 256 queries a head
-    int bias_form;  // kBiasNone, kBiasSlope or kBiasLine
-    int scaled;     // scores are scaled before the maximum (cap, bias, or a scale that is not positive)
-    int wo;         // widest copies (bytes) of out
+    int64_t items;   // (sequence, head, 256 queries)
+    int tiles;       // of 256 queries a head
+    int head_major;  // blocks walk runs of items of one head (a table in shared memory), else long ones first
+    int bias_form;
+    int scaled;      // scores are scaled before the maximum (cap, bias, or a scale that is not positive)
+    int wo;          // widest stores (bytes) of out
+    int table_st;    // kBiasGridDirect: row stride of the table in shared memory
+    int words;       // documents: 32-tile words a bit set has room for
     int *err;
 };
 
@@ -44,13 +51,24 @@ template <int DP> struct TcCfg {
     static constexpr int TILE = 128 * DP * 2;          // a tile of queries, keys or values
     static constexpr int Q = 0, K = 2 * TILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
     static constexpr int BARS = SCRATCH + 8 * 256 * 4;  // attend_row's queries, a warp each
-    static constexpr int NBAR = 2 + 4 * ST + 6;
-    static constexpr int BITS = BARS + NBAR * 8 + 16;
-    // bits: four words (seen and whole, of both query tiles) for every 32 key tiles
-    static int smem(const AttnDev &p)
+    static constexpr int NBAR = 4 + 4 * ST + 6 + 4;
+    static constexpr int MORE = BARS + NBAR * 8 + 16;
+    // behind: the bit sets (two, four words each for every 32 key tiles: seen and whole, of both query
+    // tiles), or the table (one a softmax warpgroup) and its keys' places
+    static int bit_words(const ajib_attn *op) { return op->q_doc ? (op->lk + kTcKeys * 32 - 1) / (kTcKeys * 32) : 0; }
+    // Rows of the table start table_stride apart, so that the 32 queries of a warp, neighbours on the
+    // grid, read 32 different banks.
+    static int table_stride(const ajib_attn *op)
     {
-        const int words = p.q_doc ? (p.lk + kTcKeys * 32 - 1) / (kTcKeys * 32) : 0;
-        return BITS + words * 16 + 1024;  // + the alignment of the first tile
+        const int n = 2 * op->reach_x + 1;
+        return n + ((op->grid_w - n) % 32 + 32) % 32;
+    }
+    static int64_t smem(const ajib_attn *op)
+    {
+        int64_t n = MORE + 1024 + (int64_t)bit_words(op) * 32;  // 1024: the alignment of the first tile
+        if (op->bias == AJIB_BIAS_TABLE && op->grid_w)
+            n += 2 * ((int64_t)table_stride(op) * (2 * op->reach_y + 1) * 4 + 16) + ((op->lk + 127) / 128 * 128) * 4;
+        return n;
     }
 };
 
@@ -70,6 +88,14 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(int N, boo
     const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (type << 7) | (type << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
+}
+// One lane of a converged warp. (Told by a lane number instead, the compiler takes the operands of the
+// branch's products and copies for divergent, and each issue costs 140 cycles instead of a few.)
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+    return r != 0;
 }
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
@@ -94,8 +120,143 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v)
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
+// Two fp32 operations an instruction.
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b)
+{
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_out(F2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c)
+{
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b)
+{
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b)
+{
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // The lowest n bits of a word, n of any sign or size.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
+
+// One item's queries and keys, worked out alike by every role.
+struct TcItem {
+    int b, h, row0, qn, kn;
+    bool both;                 // there are queries in the second tile
+    int t0, t1;                // key tiles that any query sees
+    int before, before_whole;  // tiles below are seen for their prefix, in part / whole
+    int full;                  // tiles below hold 128 keys
+    // key tiles [from, to) are seen by some, [whole_from, whole_to) by every query of a tile
+    int from0, to0, whole_from0, whole_to0, from1, to1, whole_from1, whole_to1;
+};
+
+__device__ __forceinline__ void tile_range(const AttnDev &p, int first, int last, int kn, int &from, int &to, int &whole_from,
+                                           int &whole_to)
+{
+    const bool no_left = p.left == INT_MAX / 2, no_right = p.right == INT_MAX / 2;
+    from = no_left ? 0 : max(first - p.left, 0) / kTcKeys;
+    to = (max(no_right ? kn : min(kn, last + p.right + 1), 0) + kTcKeys - 1) / kTcKeys;
+    whole_from = no_left ? 0 : (max(last - p.left, 0) + kTcKeys - 1) / kTcKeys;
+    whole_to = no_right ? INT_MAX : max(first + p.right + 1, 0) / kTcKeys;
+}
+
+__device__ __forceinline__ bool item_of(const AttnDev &p, int b, int h, int tile, TcItem &x)
+{
+    x.b = b;
+    x.h = h;
+    x.qn = q_count(p, x.b);
+    x.kn = k_count(p, x.b);
+    x.row0 = tile * 256;
+    if (x.row0 >= x.qn) return false;
+    const int shift = p.align_end ? x.kn - x.qn : 0;
+    const int pre = p.prefix ? min(max(__ldg(p.prefix + x.b), 0), x.kn) : 0;
+    x.both = x.row0 + 128 < x.qn;
+    const int first = x.row0 + shift, last = min(x.row0 + 256, x.qn) - 1 + shift;
+    tile_range(p, first, x.both ? first + 127 : last, x.kn, x.from0, x.to0, x.whole_from0, x.whole_to0);
+    tile_range(p, first + 128, last, x.kn, x.from1, x.to1, x.whole_from1, x.whole_to1);
+    if (!x.both) x.to1 = 0;
+    x.before = (pre + kTcKeys - 1) / kTcKeys;
+    x.before_whole = pre / kTcKeys;
+    x.full = x.kn / kTcKeys;
+    x.t0 = x.before ? 0 : x.both ? min(x.from0, x.from1) : x.from0;
+    x.t1 = max(max(x.before, x.to0), x.to1);
+    return true;
+}
+
+// The items of a block in turn: a run of them (head_major), or one of each row of gridDim.x, every
+// second row backwards, which evens out a triangle.
+struct TcWalk {
+    uint32_t at, end;
+    int k, b, h, tile;
+    __device__ __forceinline__ void start(const TcDev &P)
+    {
+        at = 0;
+        end = (uint32_t)P.items;
+        k = b = h = tile = 0;
+        if (P.head_major) {
+            at = (uint32_t)(P.items * blockIdx.x / gridDim.x);
+            end = (uint32_t)(P.items * (blockIdx.x + 1) / gridDim.x);
+            tile = at % P.tiles;
+            b = at / P.tiles;
+            h = b / P.a.batch;
+            b -= h * P.a.batch;
+        }
+    }
+    __device__ __forceinline__ bool next(const TcDev &P, TcItem &x)
+    {
+        const AttnDev &p = P.a;
+        while (at < end) {
+            bool found;
+            if (P.head_major) {
+                found = item_of(p, b, h, tile, x);
+                at++;
+                if (++tile == P.tiles) {
+                    tile = 0;
+                    if (++b == p.batch) {
+                        b = 0;
+                        h++;
+                    }
+                }
+            } else {
+                // the last queries of a prompt, which see most keys, first; heads that share keys side by side
+                uint32_t item = at + (k++ & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                at += gridDim.x;
+                if (item >= end) continue;
+                const uint32_t row = item / p.hq, last = row / p.batch;
+                found = item_of(p, row - last * p.batch, item - row * p.hq, P.tiles - 1 - (int)last, x);
+            }
+            if (found) return true;
+        }
+        return false;
+    }
+};
+
+// Whether some query of tile q sees a key of tile t. bits: the item's documents, or NULL.
+__device__ __forceinline__ bool tc_active(const TcItem &x, const uint32_t *bits, int q, int t)
+{
+    const bool reach = t < x.before ? !q || x.both : q ? t >= x.from1 && t < x.to1 : t >= x.from0 && t < x.to0;
+    return reach && !(bits && !(bits[4 * (t / 32 - x.t0 / 32) + q] >> (t & 31) & 1));
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -105,30 +266,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     using C = TcCfg<DP>;
     const AttnDev &p = P.a;
     extern __shared__ char sm_raw[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-    // ---- which queries and keys (the last queries of a prompt, which see most, first) ----
-    const int64_t bhs = (int64_t)p.batch * p.hq;
-    const int tile = P.tiles - 1 - (int)(blockIdx.x / bhs);
-    const int bh = (int)(blockIdx.x % bhs), b = bh / p.hq, h = bh - b * p.hq;
-    const int qn = q_count(p, b), kn = k_count(p, b), row0 = tile * 256;
-    if (row0 >= qn) return;
-    const int shift = p.align_end ? kn - qn : 0;
-    const int pre = p.prefix ? __ldg(p.prefix + b) : 0;
-    const int first0 = row0 + shift, last1 = min(row0 + 256, qn) - 1 + shift;
-    int key_lo, key_hi;
-    reach_of(p, first0, last1, pre, kn, key_lo, key_hi);
-    const int t0 = key_lo / kTcKeys, t1 = (max(key_hi, key_lo) + kTcKeys - 1) / kTcKeys;
-    const bool both = row0 + 128 < qn;
-    const int last0 = both ? first0 + 127 : last1, first1 = first0 + 128;
-
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     char *const sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     const uint32_t s0 = smem_u32(sm);
     const uint32_t bars = s0 + C::BARS;
-    const uint32_t q_full = bars, k_full = bars + 16, k_empty = k_full + 8 * C::ST, v_full = k_empty + 8 * C::ST,
-                   v_empty = v_full + 8 * C::ST, s_full = v_empty + 8 * C::ST, p_full = s_full + 16, o_full = p_full + 16;
+    const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * C::ST,
+                   v_full = k_empty + 8 * C::ST, v_empty = v_full + 8 * C::ST, s_full = v_empty + 8 * C::ST,
+                   p_full = s_full + 16, o_full = p_full + 16, bits_full = o_full + 16, bits_empty = bits_full + 16;
     uint32_t *const tmem_at = (uint32_t *)(sm + C::BARS + C::NBAR * 8);
-    uint32_t *const bits = (uint32_t *)(sm + C::BITS);
+    uint32_t *const bit_sets = (uint32_t *)(sm + C::MORE);
 
     if (warp == 9) {
         tmem_alloc(smem_u32(tmem_at), 512);
@@ -136,377 +282,498 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tma_prefetch_desc(&mq);
         tma_prefetch_desc(&mk);
         tma_prefetch_desc(&mv);
-        for (int i = 0; i < C::NBAR - 6; i++) mbar_init(bars + 8 * i, 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 4);  // one arrival a softmax warp
-            mbar_init(o_full + 8 * i, 1);
-        }
+        for (uint32_t x = bars; x < bits_empty + 16; x += 8)
+            mbar_init(x, x >= bits_empty ? 10 : x >= bits_full ? 2 : x >= p_full && x < o_full ? 4 : 1);
         fence_mbar_init();
-    }
-    const int *const docs = p.k_doc ? p.k_doc + (int64_t)(b % p.doc_rows) * p.lk : nullptr;
-    const int word0 = t0 / 32;
-    if (docs) {
-        // which key tiles hold a document of each query tile, and which nothing but its only one
-        const int *qd = p.q_doc + (int64_t)(b % p.doc_rows) * p.lq;
-        int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            for (int i = row0 + 128 * x + lane; i < min(row0 + 128 * x + 128, qn); i += 32) {
-                const int id = __ldg(qd + i);
-                lo[x] = min(lo[x], id);
-                hi[x] = max(hi[x], id);
-            }
-            lo[x] = __reduce_min_sync(0xffffffffu, lo[x]);
-            hi[x] = __reduce_max_sync(0xffffffffu, hi[x]);
-        }
-        for (int w = word0 + warp; w * 32 < t1; w += kTcThreads / 32) {
-            int klo = INT_MAX, khi = INT_MIN;
-            // the warp reads a tile together, lane l keeps tile l's range
-            for (int x = 0; x < 32; x++) {
-                const int t = w * 32 + x;
-                if (t < t0 || t >= t1) continue;
-                int a = INT_MAX, z = INT_MIN;
-#pragma unroll
-                for (int y = 0; y < kTcKeys / 32; y++) {
-                    const int j = t * kTcKeys + y * 32 + lane;
-                    if (j < kn) {
-                        const int id = __ldg(docs + j);
-                        a = min(a, id);
-                        z = max(z, id);
-                    }
-                }
-                a = __reduce_min_sync(0xffffffffu, a);
-                z = __reduce_max_sync(0xffffffffu, z);
-                if (lane == x) klo = a, khi = z;
-            }
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo[x], 0) <= khi && klo <= hi[x]);
-                const uint32_t whole = __ballot_sync(0xffffffffu, lo[x] >= 0 && lo[x] == hi[x] && klo == lo[x] && khi == lo[x]);
-                if (lane == 0) {
-                    bits[4 * (w - word0) + x] = seen;
-                    bits[4 * (w - word0) + 2 + x] = whole;
-                }
-            }
-        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_at;
-
-    const bool no_left = p.left == INT_MAX / 2, no_right = p.right == INT_MAX / 2;
-    // Whether some query of tile q sees a key of tile t, and whether every one sees all of them.
-    auto active = [&](int q, int t) {
-        const int j = t * kTcKeys;
-        if ((q && !both) || j >= kn) return false;
-        if (docs && !(bits[4 * (t / 32 - word0) + q] >> (t & 31) & 1)) return false;
-        return j < pre || ((no_left || j + kTcKeys - 1 >= (q ? first1 : first0) - p.left) &&
-                           (no_right || j <= (q ? last1 : last0) + p.right));
-    };
-    auto whole = [&](int q, int t) {
-        const int j = t * kTcKeys, end = j + kTcKeys;
-        if (end > kn) return false;
-        if (docs && !(bits[4 * (t / 32 - word0) + 2 + q] >> (t & 31) & 1)) return false;
-        return end <= pre || ((no_left || j >= (q ? last1 : last0) - p.left) &&
-                              (no_right || end - 1 <= (q ? first1 : first0) + p.right));
-    };
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+    const bool documents = p.q_doc != nullptr;
+    TcWalk walk;
+    TcItem x;
+    walk.start(P);
+    int turn = 0;  // items so far (their bit sets alternate)
+    bool ok = true;
+    auto bits_of = [&](int n) { return documents ? bit_sets + (n & 1) * P.words * 4 : nullptr; };
 
     // 384 threads of 168 registers: the softmax warps take 216 (a row of 128 scores and more), 72 stay
-    // for the copies, the products and two idle warps.
+    // for the copies, the products and the documents.
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8) {
             // ---- copies ----
-            if (lane == 0) {
-                const int g = h / p.group;
-                int n = 0;
-                bool ok = true;
-                for (int t = t0; t < t1 && ok; t++) {
-                    if (!active(0, t) && !active(1, t)) continue;
-                    const int st = n % C::ST;
-                    const uint32_t parity = ((n / C::ST) & 1) ^ 1;
-                    if (n == 0) {
-                        mbar_arrive_expect_tx(q_full, C::TILE);
-                        for (int x = 0; x < DP / 64; x++) tma_load_4d(s0 + C::Q + x * 16384, &mq, q_full, 64 * x, row0, h, b);
-                    }
-                    if (!(ok = mbar_wait(k_empty + 8 * st, parity, P.err, 201))) break;
-                    mbar_arrive_expect_tx(k_full + 8 * st, C::TILE);
-                    for (int x = 0; x < DP / 64; x++)
-                        tma_load_4d(s0 + C::K + st * C::TILE + x * 16384, &mk, k_full + 8 * st, 64 * x, t * kTcKeys, g, b);
-                    if (n == 0 && both) {
-                        mbar_arrive_expect_tx(q_full + 8, C::TILE);
-                        for (int x = 0; x < DP / 64; x++)
-                            tma_load_4d(s0 + C::Q + C::TILE + x * 16384, &mq, q_full + 8, 64 * x, row0 + 128, h, b);
-                    }
-                    if (!(ok = mbar_wait(v_empty + 8 * st, parity, P.err, 202))) {
+            if (elect_one()) {
+                int n = 0, nq[2] = {0, 0};
+                bool v_here = true;  // whether the last keys' values were asked for as well
+                for (; ok && walk.next(P, x); turn++) {
+                    const uint32_t *bits = bits_of(turn);
+                    if (bits && !(ok = mbar_wait(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
+                    const int g = x.h / p.group;
+                    bool q_here[2] = {false, false};
+                    auto queries = [&](int q) {
+                        if (q_here[q] || !(ok = mbar_wait(q_empty + 8 * q, (nq[q] & 1) ^ 1, P.err, 200))) return;
+                        mbar_arrive_expect_tx(q_full + 8 * q, C::TILE);
+                        for (int y = 0; y < DP / 64; y++)
+                            tma_load_4d(s0 + C::Q + q * C::TILE + y * 16384, &mq, q_full + 8 * q, 64 * y, x.row0 + 128 * q, x.h,
+                                        x.b);
+                        q_here[q] = true;
+                        nq[q]++;
+                    };
+                    for (int t = x.t0; t < x.t1 && ok; t++) {
+                        const bool act[2] = {tc_active(x, bits, 0, t), tc_active(x, bits, 1, t)};
+                        if (!act[0] && !act[1]) continue;
+                        const int st = n % C::ST;
+                        const uint32_t parity = ((n / C::ST) & 1) ^ 1;
+                        if (act[0]) queries(0);
+                        if (!ok || !(ok = mbar_wait(k_empty + 8 * st, parity, P.err, 201))) break;
+                        mbar_arrive_expect_tx(k_full + 8 * st, C::TILE);
+                        for (int y = 0; y < DP / 64; y++)
+                            tma_load_4d(s0 + C::K + st * C::TILE + y * 16384, &mk, k_full + 8 * st, 64 * y, t * kTcKeys, g, x.b);
                         n++;
-                        break;
+                        v_here = false;
+                        if (act[1]) queries(1);
+                        if (!ok || !(ok = mbar_wait(v_empty + 8 * st, parity, P.err, 202))) break;
+                        mbar_arrive_expect_tx(v_full + 8 * st, C::TILE);
+                        for (int y = 0; y < DP / 64; y++)
+                            tma_load_4d(s0 + C::V + st * C::TILE + y * 16384, &mv, v_full + 8 * st, 64 * y, t * kTcKeys, g, x.b);
+                        v_here = true;
                     }
-                    mbar_arrive_expect_tx(v_full + 8 * st, C::TILE);
-                    for (int x = 0; x < DP / 64; x++)
-                        tma_load_4d(s0 + C::V + st * C::TILE + x * 16384, &mv, v_full + 8 * st, 64 * x, t * kTcKeys, g, b);
-                    n++;
+                    if (bits) mbar_arrive(bits_empty + 8 * (turn & 1));
                 }
                 // every copy has landed before the block ends, also where a wait gave up
-                if (n) {
-                    mbar_wait(q_full, 0, P.err, 203);
-                    if (both) mbar_wait(q_full + 8, 0, P.err, 203);
-                }
+#pragma unroll
+                for (int q = 0; q < 2; q++)
+                    if (nq[q]) mbar_wait(q_full + 8 * q, (nq[q] - 1) & 1, P.err, 203);
                 for (int i = max(0, n - C::ST); i < n; i++) {
                     mbar_wait(k_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 204);
-                    if (ok || i < n - 1) mbar_wait(v_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 205);
+                    if (v_here || i < n - 1) mbar_wait(v_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 205);
                 }
             }
         } else if (warp == 9) {
             // ---- products ----
-            constexpr uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(DP, true);
-            bool pend[2] = {false, false}, acc[2] = {false, false}, q_here[2] = {false, false}, ok = true;
-            uint32_t p_phase[2] = {0, 0};
-            int n = 0, t_prev = 0;
-            // O_q += P_q V of the previous key tile
-            auto values = [&](int q, bool &v_here) {
-                const int st = (n - 1) % C::ST;
-                const uint32_t vs = s0 + C::V + st * C::TILE;
-                if (!v_here) {
-                    if (!mbar_wait_warp(v_full + 8 * st, ((n - 1) / C::ST) & 1, P.err, 206)) return false;
-                    const int live = kn - t_prev * kTcKeys;
-                    if (live < kTcKeys && kn < p.lk) {
-                        // values behind the last key may be anything: zeros, as 0 * NaN is NaN
-                        for (int i = lane; i < (kTcKeys - live) * (DP / 8); i += 32) {
-                            const int r = live + i / (DP / 8), c = i % (DP / 8);
-                            *reinterpret_cast<uint4 *>(sm + C::V + st * C::TILE + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
-                    v_here = true;
-                }
-                if (!mbar_wait_warp(p_full + 8 * q, p_phase[q], P.err, 207)) return false;
-                p_phase[q] ^= 1;
-                tc_fence_after();
-                if (lane == 0) {
-#pragma unroll
-                    for (int kk = 0; kk < kTcKeys / 16; kk++)
-                        mma_f16_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * kk, swizzled_desc(vs + kk * 2048, 16384), id_o,
-                                   acc[q] || kk > 0);
-                }
-                acc[q] = true;
-                return true;
-            };
-            for (int t = t0; t < t1 && ok; t++) {
-                const bool act[2] = {active(0, t), active(1, t)};
-                if (!act[0] && !act[1]) continue;
-                const int st = n % C::ST;
-                const uint32_t ks = s0 + C::K + st * C::TILE;
-                bool v_here = false, k_here = false;
-                for (int q = 0; q < 2 && ok; q++) {
-                    if (pend[q] && !(ok = values(q, v_here))) break;
-                    if (act[q]) {
-                        if (!k_here && !(ok = mbar_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208))) break;
-                        k_here = true;
-                        if (!q_here[q] && !(ok = mbar_wait_warp(q_full + 8 * q, 0, P.err, 209))) break;
-                        q_here[q] = true;
-                        if (lane == 0) {
-                            const uint32_t qs = s0 + C::Q + q * C::TILE;
-#pragma unroll
-                            for (int kk = 0; kk < DP / 16; kk++) {
-                                const uint32_t at = (kk >> 2) * 16384 + (kk & 3) * 32;
-                                mma_f16(tmem + 128 * q, swizzled_desc(qs + at, 16), swizzled_desc(ks + at, 16), id_s, kk > 0, 0);
+            // N of P V: the components, in sixteens; k of Q K^T likewise
+            const int dn = (p.d + 15) / 16 * 16;
+            const uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(dn, true);
+            uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+            int n = 0;
+            for (; ok && walk.next(P, x); turn++) {
+                const uint32_t *bits = bits_of(turn);
+                if (bits && !(ok = mbar_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
+                bool pend[2] = {false, false}, acc[2] = {false, false}, q_here[2] = {false, false};
+                int t_prev = 0;
+                bool prev = false;  // a key tile of this item has gone before
+                // O_q += P_q V of the key tile before
+                auto values = [&](int q, bool &v_here) {
+                    const int st = (n - 1) % C::ST;
+                    const uint32_t vs = s0 + C::V + st * C::TILE;
+                    if (!v_here) {
+                        if (!mbar_wait_warp(v_full + 8 * st, ((n - 1) / C::ST) & 1, P.err, 206)) return false;
+                        const int live = x.kn - t_prev * kTcKeys;
+                        if (live < kTcKeys && x.kn < p.lk) {
+                            // values behind the last key may be anything: zeros, as 0 * NaN is NaN
+                            for (int i = lane; i < (kTcKeys - live) * (DP / 8); i += 32) {
+                                const int r = live + i / (DP / 8), c = i % (DP / 8);
+                                *reinterpret_cast<uint4 *>(sm + C::V + st * C::TILE + (c >> 3) * 16384 + r * 128 +
+                                                           (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                             }
-                            mma_commit(s_full + 8 * q);
+                            fence_proxy_async();
+                            __syncwarp();
                         }
+                        v_here = true;
                     }
-                    pend[q] = act[q];
+                    if (!mbar_wait_warp(p_full + 8 * q, p_phase[q], P.err, 207)) return false;
+                    p_phase[q] ^= 1;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t vd = swizzled_desc(vs, 16384);
+#pragma unroll
+                        for (int kk = 0; kk < kTcKeys / 16; kk++)
+                            mma_f16_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * kk, vd + (kk * 2048 >> 4), id_o,
+                                       acc[q] || kk > 0);
+                    }
+                    acc[q] = true;
+                    return true;
+                };
+                for (int t = x.t0; t < x.t1 && ok; t++) {
+                    const bool act[2] = {tc_active(x, bits, 0, t), tc_active(x, bits, 1, t)};
+                    if (!act[0] && !act[1]) continue;
+                    const int st = n % C::ST;
+                    const uint32_t ks = s0 + C::K + st * C::TILE;
+                    bool v_here = false, k_here = false;
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        if (!ok) break;
+                        if (pend[q] && !(ok = values(q, v_here))) break;
+                        if (act[q]) {
+                            if (!q_here[q]) {
+                                if (!(ok = mbar_wait_warp(q_full + 8 * q, q_phase[q], P.err, 209))) break;
+                                q_phase[q] ^= 1;
+                                q_here[q] = true;
+                            }
+                            if (!k_here && !(ok = mbar_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208))) break;
+                            k_here = true;
+                            if (elect_one()) {
+                                const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::TILE, 16), kd = swizzled_desc(ks, 16);
+#pragma unroll
+                                for (int kk = 0; kk < DP / 16; kk++) {
+                                    const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                                    if (kk * 16 < p.d) mma_f16(tmem + 128 * q, qd + at, kd + at, id_s, kk > 0, 0);
+                                }
+                                mma_commit(s_full + 8 * q);
+                            }
+                        }
+                        pend[q] = act[q];
+                    }
+                    if (ok && elect_one()) {
+                        mma_commit(k_empty + 8 * st);
+                        if (prev) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
+                    }
+                    __syncwarp();
+                    t_prev = t;
+                    prev = true;
+                    n++;
                 }
-                if (ok && lane == 0) {
-                    mma_commit(k_empty + 8 * st);
-                    if (n > 0) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
+                // the queries are free when the last scores are there; the outputs of each tile as it ends
+                if (ok && elect_one()) {
+                    if (q_here[0]) mma_commit(q_empty);
+                    if (q_here[1]) mma_commit(q_empty + 8);
+                }
+                bool v_here = false;
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    if (ok && pend[q]) ok = values(q, v_here);
+                    if (ok && acc[q] && elect_one()) mma_commit(o_full + 8 * q);
+                }
+                if (ok && prev && elect_one()) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
+                if (bits && lane == 0) mbar_arrive(bits_empty + 8 * (turn & 1));
+                __syncwarp();
+            }
+            // no product is in flight when the block ends (the softmax warps do not wait where a wait gave up)
+            if (!ok) {
+                if (elect_one()) {
+                    mma_commit(o_full);
+                    mma_commit(o_full + 8);
                 }
                 __syncwarp();
-                t_prev = t;
-                n++;
+                for (int i = 0; i < 2; i++) mbar_wait_warp(o_full, i, P.err, 212);
             }
-            bool v_here = false;
-            for (int q = 0; q < 2 && ok; q++)
-                if (pend[q]) ok = values(q, v_here);
-            if (lane == 0) {
-                mma_commit(o_full);
-                mma_commit(o_full + 8);
+        } else if (documents) {
+            // ---- documents: which key tiles hold one of a query tile's, and which nothing but its only one ----
+            for (; ok && walk.next(P, x); turn++) {
+                if (!(ok = mbar_wait_warp(bits_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214))) break;
+                uint32_t *bits = bit_sets + (turn & 1) * P.words * 4;
+                const int *qd = p.q_doc + (int64_t)(x.b % p.doc_rows) * p.lq, *kd = p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk;
+                int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const int i = x.row0 + 32 * y + lane;
+                    if (i < x.qn) {
+                        const int id = __ldg(qd + i);
+                        lo[y >> 2] = min(lo[y >> 2], id);
+                        hi[y >> 2] = max(hi[y >> 2], id);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    lo[q] = __reduce_min_sync(0xffffffffu, lo[q]);
+                    hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
+                }
+                const int word0 = x.t0 / 32;
+                for (int w = word0 + warp - 10; w * 32 < x.t1; w += 2) {
+                    int klo = INT_MAX, khi = INT_MIN;
+                    for (int y = max(x.t0 - w * 32, 0); y < min(x.t1 - w * 32, 32); y += 4) {
+                        // four tiles' loads in flight; lane l keeps tile l's range
+                        int a[4], z[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            a[u] = INT_MAX, z[u] = INT_MIN;
+#pragma unroll
+                            for (int v = 0; v < kTcKeys / 32; v++) {
+                                const int j = (w * 32 + y + u) * kTcKeys + v * 32 + lane;
+                                if (j < x.kn) {
+                                    const int id = __ldg(kd + j);
+                                    a[u] = min(a[u], id);
+                                    z[u] = max(z[u], id);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int aa = __reduce_min_sync(0xffffffffu, a[u]), zz = __reduce_max_sync(0xffffffffu, z[u]);
+                            if (lane == y + u) klo = aa, khi = zz;
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo[q], 0) <= khi && klo <= hi[q]);
+                        const uint32_t only =
+                            __ballot_sync(0xffffffffu, lo[q] >= 0 && lo[q] == hi[q] && klo == lo[q] && khi == lo[q]);
+                        if (lane == 0) {
+                            bits[4 * (w - word0) + q] = seen;
+                            bits[4 * (w - word0) + 2 + q] = only;
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bits_full + 8 * (turn & 1));
             }
-            __syncwarp();
-            mbar_wait_warp(o_full, 0, P.err, 212);  // no product is in flight when the block ends
         }
     } else {
         // ---- softmax ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int q = warp >> 2, r_in = (warp & 3) * 32 + lane, i = row0 + 128 * q + r_in;
+        const int q = warp >> 2, r_in = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + 128 * q, o_at = tmem + lanes + 256 + 128 * q;
-        const bool there = i < qn;
-        const Query r = query_of(p, b, h, min(i, qn - 1), qn, kn);
         const float sc = P.scaled ? 1.f : p.scale;
-        float m = -INFINITY, l = 0.f;  // m: in the units of the scores; times sc it is base 2
-        uint32_t phase = 0;
-        bool any = false, ok = true;
-        for (int t = t0; t < t1; t++) {
-            if (!active(q, t)) continue;
-            if (!(ok = mbar_wait_warp(s_full + 8 * q, phase, P.err, 210))) break;
-            phase ^= 1;
-            tc_fence_after();
-            float s[128];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, s + 32 * c);
-            tmem_wait_ld();
-            const int j0 = t * kTcKeys;
-            if (P.scaled) {
-                if (p.cap_out > 0.f) {
-#pragma unroll
-                    for (int c = 0; c < 128; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 128; c++) s[c] *= p.scale;
-                }
-                if (P.bias_form == kBiasSlope) {
-                    const float d0 = (float)(r.at - j0);
-#pragma unroll
-                    for (int c = 0; c < 128; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
-                } else if (P.bias_form == kBiasLine) {
-#pragma unroll
-                    for (int c = 0; c < 128; c++) s[c] += table_bias(p, r, 0, j0 + c);
-                }
+        const bool grid = P.bias_form == kBiasGridDirect, quads = p.grid_w % 4 == 0;
+        const int table_n = grid ? P.table_st * (2 * p.reach_y + 1) : 0;
+        float *const table = (float *)(sm + C::MORE + P.words * 32) + q * (table_n + 3) / 4 * 4;
+        int *const places = (int *)((float *)(sm + C::MORE + P.words * 32) + 2 * ((table_n + 3) / 4 * 4));
+        int table_h = -1;
+        if (grid) {
+            // where a key's (grids a multiple of 4 wide: four keys') entry of the table is, from its query's;
+            // behind the last key: the first's, which is masked
+            for (int j = tid; j < (p.lk + 127) / 128 * 128; j += 256) {
+                const int jj = j < p.lk ? j : 0, y = jj / p.grid_w, at = y * P.table_st + jj - y * p.grid_w;
+                if (!quads)
+                    places[j] = at;
+                else if (j % 4 == 0)
+                    places[j / 4] = at;
             }
-            if (!whole(q, t)) {
-                // a bit a key: [0, before) or [lo, hi), below end, of this query's document
-                const int lo = max(r.lo, 0) - j0, hi = min(r.hi == INT_MAX ? INT_MAX : r.hi - j0, 127) + 1;
-                const int before = min(r.pre - j0, 128), end = min(kn - j0, 128);
-                uint32_t seen[4];
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    seen[w] = (bits_below(hi - 32 * w) & ~bits_below(lo - 32 * w)) | bits_below(before - 32 * w);
-                    seen[w] &= bits_below(end - 32 * w);
-                    if (docs && seen[w]) {
-                        uint32_t same = 0;
-#pragma unroll 4
-                        for (int c = 0; c < 32; c++)
-                            same |= (uint32_t)(__ldg(docs + min(j0 + 32 * w + c, kn - 1)) == r.doc) << c;
-                        seen[w] &= same;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 128; c++) s[c] = seen[c >> 5] >> (c & 31) & 1 ? s[c] : -INFINITY;
-            }
-            float top[4];
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                top[x] = s[x];
-#pragma unroll
-                for (int c = 4 + x; c < 128; c += 4) top[x] = fmaxf(top[x], s[c]);
-            }
-            const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            // (m is -inf until a row has seen a key)
-            if (__any_sync(0xffffffffu, now * sc > m * sc + 8.f || (m == -INFINITY && now > m))) {
-                const float to = fmaxf(m, now), alpha = exp2_fast((m - (to == -INFINITY ? 0.f : to)) * sc);
-                if (any) {
-                    for (int c = 0; c < DP; c += 32) {
-                        float o[32];
-                        tmem_ld32(o_at + c, o);
-                        tmem_wait_ld();
-                        uint32_t w[2][16];
-#pragma unroll
-                        for (int x = 0; x < 32; x++) w[x >> 4][x & 15] = __float_as_uint(o[x] * alpha);
-                        tmem_st16(o_at + c, w[0]);
-                        tmem_st16(o_at + c + 16, w[1]);
-                    }
-                }
-                l *= m == -INFINITY ? 0.f : alpha;
-                m = to;
-            }
-            any = true;
-            const float base = m == -INFINITY ? 0.f : m * sc;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t w[16];
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const float a = exp2_fast(fmaf(s[32 * c + 2 * x], sc, -base)),
-                                z = exp2_fast(fmaf(s[32 * c + 2 * x + 1], sc, -base));
-                    sum[(2 * x) & 3] += a;
-                    sum[(2 * x + 1) & 3] += z;
-                    w[x] = MmaOp<T>::pack(a, z);
-                }
-                tmem_st16(s_at + 16 * c, w);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * q);
+            named_bar_sync(3, 256);
         }
+        uint32_t s_phase = 0, o_phase = 0;
+        for (; walk.next(P, x); turn++) {
+            if (grid && table_h != x.h) {
+                // (a warp whose wait gave up still comes to these barriers)
+                named_bar_sync(1 + q, 128);
+                const float *src = p.bias_data + (int64_t)x.h * (2 * p.reach_y + 1) * (2 * p.reach_x + 1);
+                for (int e = tid & 127; e < table_n; e += 128) {
+                    const int y = e / P.table_st, c = e - y * P.table_st;
+                    if (c <= 2 * p.reach_x) table[e] = __ldg(src + y * (2 * p.reach_x + 1) + c) * kLog2e;
+                }
+                named_bar_sync(1 + q, 128);
+                table_h = x.h;
+            }
+            if (!ok) continue;
+            const uint32_t *bits = bits_of(turn);
+            if (bits && !(ok = mbar_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) continue;
+            const int i = x.row0 + 128 * q + r_in;
+            const bool there = i < x.qn;
+            const Query r = query_of(p, x.b, x.h, min(i, x.qn - 1), x.qn, x.kn);
+            const int *const docs = documents ? p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk : nullptr;
+            const float *const mine = table + (p.reach_y - r.y) * P.table_st + p.reach_x - r.x;
+            const int from = q ? x.from1 : x.from0, to = q ? x.to1 : x.to0, before = q && !x.both ? 0 : x.before;
+            const int whole_from = q ? x.whole_from1 : x.whole_from0, whole_to = q ? x.whole_to1 : x.whole_to0;
+            float m = -INFINITY, l = 0.f;  // m: in the units of the scores; times sc it is base 2
+            bool any = false;
+            for (int t = x.t0; t < x.t1; t++) {
+                if (!(t < before || (t >= from && t < to))) continue;
+                bool all = t < x.full && (t < x.before_whole || (t >= whole_from && t < whole_to));
+                if (bits) {
+                    const uint32_t *word = bits + 4 * (t / 32 - x.t0 / 32) + q;
+                    if (!(word[0] >> (t & 31) & 1)) continue;
+                    all = all && word[2] >> (t & 31) & 1;
+                }
+                const int j0 = t * kTcKeys;
+                int ids[4];
+                if (docs && !all) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) ids[w] = __ldg(docs + min(j0 + 32 * w + lane, x.kn - 1));
+                }
+                if (!(ok = mbar_wait_warp(s_full + 8 * q, s_phase, P.err, 210))) break;
+                s_phase ^= 1;
+                tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, s + 32 * c);
+                tmem_wait_ld();
+                if (P.scaled) {
+                    if (p.cap_out > 0.f) {
+#pragma unroll
+                        for (int c = 0; c < 128; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
+                    } else if (!grid) {
+#pragma unroll
+                        for (int c = 0; c < 128; c++) s[c] *= p.scale;
+                    }
+                    if (P.bias_form == kBiasSlope) {
+                        const float d0 = (float)(r.at - j0);
+#pragma unroll
+                        for (int c = 0; c < 128; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
+                    } else if (P.bias_form == kBiasLine) {
+#pragma unroll
+                        for (int c = 0; c < 128; c++) s[c] += table_bias(p, r, 0, j0 + c);
+                    } else if (grid) {
+                        const float f = p.cap_out > 0.f ? 1.f : p.scale;
+                        const F2 ff = f2(f, f);
+                        if (quads) {
+#pragma unroll
+                            for (int c = 0; c < 128; c += 16) {
+                                const int4 at = *reinterpret_cast<const int4 *>(places + ((j0 + c) >> 2));
+#pragma unroll
+                                for (int y = 0; y < 16; y += 2) {
+                                    const float *e = mine + (y < 4 ? at.x : y < 8 ? at.y : y < 12 ? at.z : at.w) + (y & 3);
+                                    f2_out(f2_fma(f2(s[c + y], s[c + y + 1]), ff, f2(e[0], e[1])), s[c + y], s[c + y + 1]);
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 128; c += 4) {
+                                const int4 at = *reinterpret_cast<const int4 *>(places + j0 + c);
+                                s[c] = fmaf(s[c], f, mine[at.x]);
+                                s[c + 1] = fmaf(s[c + 1], f, mine[at.y]);
+                                s[c + 2] = fmaf(s[c + 2], f, mine[at.z]);
+                                s[c + 3] = fmaf(s[c + 3], f, mine[at.w]);
+                            }
+                        }
+                    }
+                }
+                if (!all) {
+                    // a bit a key: [0, below) or [lo, hi), below end, of this query's document
+                    const int lo = max(r.lo, 0) - j0, hi = min(r.hi == INT_MAX ? INT_MAX : r.hi - j0, 127) + 1;
+                    const int below = min(r.pre - j0, 128), end = min(x.kn - j0, 128);
+                    uint32_t seen[4];
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+                        seen[w] = ((bits_below(hi - 32 * w) & ~bits_below(lo - 32 * w)) | bits_below(below - 32 * w)) &
+                                  bits_below(end - 32 * w);
+                    if (docs) {
+                        // one vote for each document among the warp's queries
+                        for (uint32_t left = 0xffffffffu; left;) {
+                            const int id = __shfl_sync(0xffffffffu, r.doc, __ffs(left) - 1);
+                            const bool same = r.doc == id;
+#pragma unroll
+                            for (int w = 0; w < 4; w++) {
+                                const uint32_t of = __ballot_sync(0xffffffffu, ids[w] == id);
+                                if (same) seen[w] &= of;
+                            }
+                            left &= ~__ballot_sync(0xffffffffu, same);
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 128; c++) s[c] = seen[c >> 5] >> (c & 31) & 1 ? s[c] : -INFINITY;
+                }
+                float top[4];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    top[y] = s[y];
+#pragma unroll
+                    for (int c = 4 + y; c < 124; c += 8) top[y] = max3(top[y], s[c], s[c + 4]);
+                    top[y] = fmaxf(top[y], s[124 + y]);
+                }
+                const float now = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+                // (m is -inf until a row has seen a key)
+                if (__any_sync(0xffffffffu, now * sc > m * sc + 8.f || (m == -INFINITY && now > m))) {
+                    const float to = fmaxf(m, now), alpha = exp2_fast((m - (to == -INFINITY ? 0.f : to)) * sc);
+                    if (any) {
+                        for (int c = 0; c < p.d; c += 32) {
+                            float o[32];
+                            tmem_ld32(o_at + c, o);
+                            tmem_wait_ld();
+                            uint32_t w[2][16];
+#pragma unroll
+                            for (int y = 0; y < 32; y++) w[y >> 4][y & 15] = __float_as_uint(o[y] * alpha);
+                            tmem_st16(o_at + c, w[0]);
+                            tmem_st16(o_at + c + 16, w[1]);
+                        }
+                    }
+                    l *= m == -INFINITY ? 0.f : alpha;
+                    m = to;
+                }
+                any = true;
+                const float base = m == -INFINITY ? 0.f : m * sc;
+                const F2 sc2 = f2(sc, sc), base2 = f2(-base, -base);
+                F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int y = 0; y < 16; y++) {
+                        float a, z;
+                        f2_out(f2_fma(f2(s[32 * c + 2 * y], s[32 * c + 2 * y + 1]), sc2, base2), a, z);
+                        a = exp2_fast(a);
+                        z = exp2_fast(z);
+                        sum[y & 1] = f2_add(sum[y & 1], f2(a, z));
+                        w[y] = MmaOp<T>::pack(a, z);
+                    }
+                    tmem_st16(s_at + 16 * c, w);
+                }
+                float la, lb;
+                f2_out(f2_add(sum[0], sum[1]), la, lb);
+                l += la + lb;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * q);
+            }
+            if (bits) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bits_empty + 8 * (turn & 1));
+            }
+            if (!ok) continue;
 
-        // ---- out ----
-        if (ok && any) ok = mbar_wait_warp(o_full + 8 * q, 0, P.err, 211);
-        if (ok && (q == 0 || both)) {
-            tc_fence_after();
+            // ---- out: a thread a row ----
+            if (any) {
+                if (!(ok = mbar_wait_warp(o_full + 8 * q, o_phase, P.err, 211))) continue;
+                o_phase ^= 1;
+                tc_fence_after();
+            }
+            if (q && !x.both) continue;
             const float f = l == 0.f ? 0.f : 1.f / l;
-            char *const mine = sm + C::Q + q * C::TILE;  // this warp's 32 rows of the queries, no longer read
+            T *const dst = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)i * p.ot;
             bool odd = false;
-            for (int c = 0; c < DP; c += 32) {
+            for (int c = 0; c < p.d; c += 32) {
                 float o[32];
                 if (any) {
                     tmem_ld32(o_at + c, o);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int x = 0; x < 32; x++) {
-                    if (!any) o[x] = 0.f;
-                    odd |= !(fabsf(o[x]) < INFINITY);
-                    o[x] = l == 0.f ? 0.f : o[x] * f;
+                for (int y = 0; y < 32; y++) {
+                    if (!any) o[y] = 0.f;
+                    if (c + y < p.d) odd |= !(fabsf(o[y]) < INFINITY);
+                    o[y] = l == 0.f ? 0.f : o[y] * f;
                 }
+                uint32_t w[16];
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int ch = (c >> 3) + x;
-                    *reinterpret_cast<uint4 *>(mine + (ch >> 3) * 16384 + r_in * 128 + (((ch & 7) ^ (r_in & 7)) << 4)) =
-                        make_uint4(MmaOp<T>::pack(o[8 * x], o[8 * x + 1]), MmaOp<T>::pack(o[8 * x + 2], o[8 * x + 3]),
-                                   MmaOp<T>::pack(o[8 * x + 4], o[8 * x + 5]), MmaOp<T>::pack(o[8 * x + 6], o[8 * x + 7]));
+                for (int y = 0; y < 16; y++) w[y] = MmaOp<T>::pack(o[2 * y], o[2 * y + 1]);
+                if (!there) continue;
+                // (d is a multiple of 8, of 16 where 32-byte stores are allowed)
+                if (P.wo == 32) {
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+                        if (c + 16 * y < p.d)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c + 16 * y),
+                                         "r"(w[8 * y]), "r"(w[8 * y + 1]), "r"(w[8 * y + 2]), "r"(w[8 * y + 3]),
+                                         "r"(w[8 * y + 4]), "r"(w[8 * y + 5]), "r"(w[8 * y + 6]), "r"(w[8 * y + 7])
+                                         : "memory");
+                } else if (P.wo == 16) {
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if (c + 8 * y < p.d)
+                            *reinterpret_cast<uint4 *>(dst + c + 8 * y) =
+                                make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 32; y++)
+                        if (c + y < p.d) dst[c + y] = from_f<T>(o[y]);
                 }
             }
-            __syncwarp();
-            // A row that is not finite again from the keys that it sees alone (0 * v of one that it does not
-            // see is NaN when v is not finite).
+            // A row that is not finite again from the keys that it sees alone (0 * v of one that it does not see
+            // is NaN when v is not finite).
             uint32_t again = p.masked ? __ballot_sync(0xffffffffu, there && odd) : 0u;
-            const int r0 = (warp & 3) * 32;
             for (; again; again &= again - 1) {
-                const int x = __ffs(again) - 1;
+                const int row = x.row0 + 128 * q + (warp & 3) * 32 + __ffs(again) - 1;
                 float rm, rl, ro[8];
-                attend_row<T>(p, b, h, row0 + 128 * q + r0 + x, qn, kn, t0 * kTcKeys, min(t1 * kTcKeys, kn),
+                attend_row<T>(p, x.b, x.h, row, x.qn, x.kn, x.t0 * kTcKeys, min(x.t1 * kTcKeys, x.kn),
                               (float *)(sm + C::SCRATCH) + warp * 256, rm, rl, ro);
                 const float rf = rl == 0.f ? 0.f : 1.f / rl;
+                T *const to = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)row * p.ot;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int c = lane + 32 * e, ch = c >> 3, row = r0 + x;
-                    if (c < p.d)
-                        *reinterpret_cast<T *>(mine + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (c & 7) * 2) =
-                            from_f<T>(rl == 0.f ? 0.f : ro[e] * rf);
-                }
-                __syncwarp();
-            }
-            T *const out = (T *)p.out + b * p.ob + h * p.oh;
-            const int per = P.wo == 16 ? 8 : P.wo == 4 ? 2 : 1, units = p.d / per;
-            for (int idx = lane; idx < 32 * units; idx += 32) {
-                const int x = idx / units, c = (idx - x * units) * per, row = r0 + x, ch = c >> 3;
-                if (row0 + 128 * q + row >= qn) break;
-                T *dst = out + (int64_t)(row0 + 128 * q + row) * p.ot + c;
-                const char *src = mine + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (c & 7) * 2;
-                if (per == 8)
-                    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
-                else if (per == 2)
-                    *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
-                else
-                    *dst = *reinterpret_cast<const T *>(src);
+                for (int e = 0; e < 4; e++)
+                    if (lane + 32 * e < p.d) to[lane + 32 * e] = from_f<T>(rl == 0.f ? 0.f : ro[e] * rf);
             }
         }
     }
