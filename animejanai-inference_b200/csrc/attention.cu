@@ -9,14 +9,13 @@
 #include <cmath>
 
 #include "attention_mma.cuh"
-#include "attention_tc.cuh"
+#include "attention_tc_run.h"
 #include "cuctx.h"
 #include "heads.h"
 
 namespace ajib {
 
 int sm_count();  // conv.cu
-int *attn_status_word();
 
 namespace {
 
@@ -34,8 +33,6 @@ struct Choice {
     int64_t rows = 0, blocks = 0;  // of a (sequence, key head); of the grid
     size_t space = 0;
 };
-
-constexpr int kMaxSmem = 227 * 1024;
 
 // Whether the table of a grid reaches every distance on it: then it is read without clamps.
 bool grid_reached(const ajib_attn *op)
@@ -72,18 +69,6 @@ bool choose(const ajib_attn *op, Choice &c)
         }
     }
     return c.blocks <= 0x7fffffff;
-}
-
-template <typename K>
-cudaError_t allow_smem(K kernel, int smem, std::atomic<uint64_t> &done)
-{
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return cudaErrorInvalidDevice;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done.load() & bit) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) done.fetch_or(bit);
-    return e;
 }
 
 template <typename T, int DP, bool KEYS>
@@ -140,19 +125,6 @@ bool map_of(CUtensorMap *m, const ajib_heads *x, int batch, int tokens, int head
     return encode(m, dtype == AJIB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x->p, dims,
                   strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <typename T, int DP>
-cudaError_t run_tc(TcDev &p, const ajib_attn *op, const CUtensorMap (&m)[3], cudaStream_t s)
-{
-    static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem(k_attn_tc<T, DP>, kMaxSmem, done);
-    if (e != cudaSuccess) return e;
-    p.words = TcCfg<DP>::bit_words(op);
-    p.table_st = TcCfg<DP>::table_stride(op);
-    const unsigned blocks = (unsigned)std::min<int64_t>(p.items, sm_count());
-    k_attn_tc<T, DP><<<blocks, kTcThreads, (int)TcCfg<DP>::smem(op), s>>>(p, m[0], m[1], m[2]);
-    return cudaGetLastError();
 }
 
 bool misaligned4(const void *p) { return ((uintptr_t)p & 3) != 0; }
@@ -286,10 +258,8 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         t.wo = rows % 32 == 0 ? 32 : m.wo;
         t.err = attn_status_word();
         if (!t.err) return AJIB_ERR_CUDA;
-        const bool f16 = op->dtype == AJIB_F16;
-        const cudaStream_t s = (cudaStream_t)stream;
-        const cudaError_t e = d <= 64 ? (f16 ? run_tc<__half, 64>(t, op, maps, s) : run_tc<__nv_bfloat16, 64>(t, op, maps, s))
-                                      : (f16 ? run_tc<__half, 128>(t, op, maps, s) : run_tc<__nv_bfloat16, 128>(t, op, maps, s));
+        const cudaError_t e = op->dtype == AJIB_F16 ? attn_tc_f16(t, op, maps, (cudaStream_t)stream)
+                                                    : attn_tc_bf16(t, op, maps, (cudaStream_t)stream);
         return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
     }
     const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(m, c, (cudaStream_t)stream)

@@ -6,9 +6,10 @@
  * copies, warp 9 the matrix products, warps 10 and 11 look up which key tiles hold which documents:
  *   S_q = Q_q K^T   (both from shared memory)       -> TMEM, 128 columns each
  *   O_q += P_q V    (P from TMEM, V from shared)    -> TMEM, DP columns each
- * P_q takes the columns of S_q: a thread holds its whole row of scores in registers before it writes
- * probabilities back, so TMEM's 512 columns hold both tiles at 128 components. The products are
- * issued P0 V, S0', P1 V, S1': while one tile's softmax runs, the other tile's products do.
+ * At 128 components P_q takes the columns of S_q (a thread holds its whole row of scores in registers
+ * before it writes probabilities back), so TMEM's 512 columns hold both tiles. The products are issued
+ * P0 V, S0', P1 V, S1': while one tile's softmax runs, the other tile's products do. Up to 64
+ * components P has columns of its own and S0', S1' go first: the softmax then never waits for them.
  *
  * The running maximum a row is scaled by only follows the true one when that has grown by more than
  * 2^8: the accumulators are rescaled rarely, and by the softmax threads themselves, at a time when
@@ -33,6 +34,10 @@ namespace ajib {
 
 constexpr int kTcThreads = 384, kTcKeys = 128;
 
+// What happens to scores beside the scale; a kernel each, as code that is jumped over costs
+// instruction fetches. kFormAny looks at the op for everything.
+enum { kFormPlain = 0, kFormCap = 1, kFormSlope = 2, kFormGrid = 3, kFormAny = 4 };
+
 struct TcDev {
     AttnDev a;
     int64_t items;   // (sequence, head, 256 queries)
@@ -51,7 +56,11 @@ template <int DP> struct TcCfg {
     static constexpr int TILE = 128 * DP * 2;          // a tile of queries, keys or values
     static constexpr int Q = 0, K = 2 * TILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
     static constexpr int BARS = SCRATCH + 8 * 256 * 4;  // attend_row's queries, a warp each
-    static constexpr int NBAR = 4 + 4 * ST + 6 + 4;
+    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 4;
+    // With up to 64 components TMEM has room for probabilities beside the scores (P at 256 + 64 q, O at
+    // 384 + 64 q): the next scores are computed as soon as the last are in registers.
+    static constexpr bool APART = DP == 64;
+    static constexpr int P_AT = APART ? 256 : 0, P_Q = APART ? 64 : 128, O_AT = APART ? 384 : 256, O_Q = APART ? 64 : 128;
     static constexpr int MORE = BARS + NBAR * 8 + 16;
     // behind: the bit sets (two, four words each for every 32 key tiles: seen and whole, of both query
     // tiles), or the table (one a softmax warpgroup) and its keys' places
@@ -258,7 +267,7 @@ __device__ __forceinline__ bool tc_active(const TcItem &x, const uint32_t *bits,
     return reach && !(bits && !(bits[4 * (t / 32 - x.t0 / 32) + q] >> (t & 31) & 1));
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int FORM>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attn_tc(const __grid_constant__ TcDev P, const __grid_constant__ CUtensorMap mq,
               const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv)
@@ -272,7 +281,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t bars = s0 + C::BARS;
     const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * C::ST,
                    v_full = k_empty + 8 * C::ST, v_empty = v_full + 8 * C::ST, s_full = v_empty + 8 * C::ST,
-                   p_full = s_full + 16, o_full = p_full + 16, bits_full = o_full + 16, bits_empty = bits_full + 16;
+                   s_empty = s_full + 16, p_full = s_empty + 16, p_empty = p_full + 16, o_full = p_empty + 16,
+                   bits_full = o_full + 16, bits_empty = bits_full + 16;
     uint32_t *const tmem_at = (uint32_t *)(sm + C::BARS + C::NBAR * 8);
     uint32_t *const bit_sets = (uint32_t *)(sm + C::MORE);
 
@@ -283,7 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tma_prefetch_desc(&mk);
         tma_prefetch_desc(&mv);
         for (uint32_t x = bars; x < bits_empty + 16; x += 8)
-            mbar_init(x, x >= bits_empty ? 10 : x >= bits_full ? 2 : x >= p_full && x < o_full ? 4 : 1);
+            mbar_init(x, x >= bits_empty ? 10 : x >= bits_full ? 2 : x >= s_empty && x < p_empty ? 4 : 1);
         fence_mbar_init();
     }
     tc_fence_before();
@@ -356,14 +366,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // N of P V: the components, in sixteens; k of Q K^T likewise
             const int dn = (p.d + 15) / 16 * 16;
             const uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(dn, true);
-            uint32_t p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+            uint32_t phase = 0;  // of p_full (bits 0, 1), q_full (2, 3) and s_empty (4, 5)
+            auto wait = [&](uint32_t bar, int bit, int code) {
+                const bool done = mbar_wait_warp(bar, phase >> bit & 1, P.err, code);
+                phase ^= 1u << bit;
+                return done;
+            };
             int n = 0;
+            uint32_t s_made = 0;  // scores computed before, by query tile: their columns are to be free again
             for (; ok && walk.next(P, x); turn++) {
                 const uint32_t *bits = bits_of(turn);
                 if (bits && !(ok = mbar_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
-                bool pend[2] = {false, false}, acc[2] = {false, false}, q_here[2] = {false, false};
+                uint32_t pend = 0, acc = 0, q_here = 0;  // by query tile
                 int t_prev = 0;
                 bool prev = false;  // a key tile of this item has gone before
+                // S_q = Q_q K^T of key tile t, the n-th
+                auto scores = [&](int q, bool &k_here) {
+                    const int st = n % C::ST;
+                    if (!(q_here >> q & 1)) {
+                        if (!wait(q_full + 8 * q, 2 + q, 209)) return false;
+                        q_here |= 1u << q;
+                    }
+                    if (!k_here && !mbar_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208)) return false;
+                    k_here = true;
+                    if (C::APART) {
+                        if (s_made >> q & 1) {
+                            if (!wait(s_empty + 8 * q, 4 + q, 215)) return false;
+                            tc_fence_after();
+                        }
+                        s_made |= 1u << q;
+                    }
+                    if (elect_one()) {
+                        const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::TILE, 16), kd = swizzled_desc(s0 + C::K + st * C::TILE, 16);
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; kk++) {
+                            const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                            if (kk * 16 < p.d) mma_f16(tmem + 128 * q, qd + at, kd + at, id_s, kk > 0, 0);
+                        }
+                        mma_commit(s_full + 8 * q);
+                    }
+                    return true;
+                };
                 // O_q += P_q V of the key tile before
                 auto values = [&](int q, bool &v_here) {
                     const int st = (n - 1) % C::ST;
@@ -383,51 +426,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         v_here = true;
                     }
-                    if (!mbar_wait_warp(p_full + 8 * q, p_phase[q], P.err, 207)) return false;
-                    p_phase[q] ^= 1;
+                    if (!wait(p_full + 8 * q, q, 207)) return false;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint64_t vd = swizzled_desc(vs, 16384);
 #pragma unroll
                         for (int kk = 0; kk < kTcKeys / 16; kk++)
-                            mma_f16_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * kk, vd + (kk * 2048 >> 4), id_o,
-                                       acc[q] || kk > 0);
+                            mma_f16_ts(tmem + C::O_AT + C::O_Q * q, tmem + C::P_AT + C::P_Q * q + 8 * kk, vd + (kk * 2048 >> 4), id_o,
+                                       (acc >> q & 1) || kk > 0);
+                        if (C::APART) mma_commit(p_empty + 8 * q);
                     }
-                    acc[q] = true;
+                    acc |= 1u << q;
                     return true;
                 };
                 for (int t = x.t0; t < x.t1 && ok; t++) {
-                    const bool act[2] = {tc_active(x, bits, 0, t), tc_active(x, bits, 1, t)};
-                    if (!act[0] && !act[1]) continue;
-                    const int st = n % C::ST;
-                    const uint32_t ks = s0 + C::K + st * C::TILE;
+                    const bool a0 = tc_active(x, bits, 0, t), a1 = tc_active(x, bits, 1, t);
+                    if (!a0 && !a1) continue;
                     bool v_here = false, k_here = false;
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        if (!ok) break;
-                        if (pend[q] && !(ok = values(q, v_here))) break;
-                        if (act[q]) {
-                            if (!q_here[q]) {
-                                if (!(ok = mbar_wait_warp(q_full + 8 * q, q_phase[q], P.err, 209))) break;
-                                q_phase[q] ^= 1;
-                                q_here[q] = true;
-                            }
-                            if (!k_here && !(ok = mbar_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208))) break;
-                            k_here = true;
-                            if (elect_one()) {
-                                const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::TILE, 16), kd = swizzled_desc(ks, 16);
-#pragma unroll
-                                for (int kk = 0; kk < DP / 16; kk++) {
-                                    const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-                                    if (kk * 16 < p.d) mma_f16(tmem + 128 * q, qd + at, kd + at, id_s, kk > 0, 0);
-                                }
-                                mma_commit(s_full + 8 * q);
-                            }
-                        }
-                        pend[q] = act[q];
+                    if (C::APART) {
+                        ok = (!a0 || scores(0, k_here)) && (!a1 || scores(1, k_here)) && (!(pend & 1) || values(0, v_here)) &&
+                             (!(pend & 2) || values(1, v_here));
+                    } else {
+                        ok = (!(pend & 1) || values(0, v_here)) && (!a0 || scores(0, k_here)) &&
+                             (!(pend & 2) || values(1, v_here)) && (!a1 || scores(1, k_here));
                     }
+                    pend = (a0 ? 1u : 0u) | (a1 ? 2u : 0u);
                     if (ok && elect_one()) {
-                        mma_commit(k_empty + 8 * st);
+                        mma_commit(k_empty + 8 * (n % C::ST));
                         if (prev) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
                     }
                     __syncwarp();
@@ -437,14 +462,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 // the queries are free when the last scores are there; the outputs of each tile as it ends
                 if (ok && elect_one()) {
-                    if (q_here[0]) mma_commit(q_empty);
-                    if (q_here[1]) mma_commit(q_empty + 8);
+                    if (q_here & 1) mma_commit(q_empty);
+                    if (q_here & 2) mma_commit(q_empty + 8);
                 }
                 bool v_here = false;
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
-                    if (ok && pend[q]) ok = values(q, v_here);
-                    if (ok && acc[q] && elect_one()) mma_commit(o_full + 8 * q);
+                    if (ok && (pend >> q & 1)) ok = values(q, v_here);
+                    if (ok && (acc >> q & 1) && elect_one()) mma_commit(o_full + 8 * q);
                 }
                 if (ok && prev && elect_one()) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
                 if (bits && lane == 0) mbar_arrive(bits_empty + 8 * (turn & 1));
@@ -525,9 +550,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int q = warp >> 2, r_in = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + 128 * q, o_at = tmem + lanes + 256 + 128 * q;
-        const float sc = P.scaled ? 1.f : p.scale;
-        const bool grid = P.bias_form == kBiasGridDirect, quads = p.grid_w % 4 == 0;
+        const uint32_t s_at = tmem + lanes + 128 * q, p_at = tmem + lanes + C::P_AT + C::P_Q * q,
+                       o_at = tmem + lanes + C::O_AT + C::O_Q * q;
+        const bool grid = FORM == kFormGrid || (FORM == kFormAny && P.bias_form == kBiasGridDirect);
+        const bool capped = FORM == kFormCap || (FORM == kFormAny && p.cap_out > 0.f);
+        const bool scaled = FORM != kFormPlain && (FORM != kFormAny || P.scaled);
+        const float sc = scaled ? 1.f : p.scale;
+        const bool quads = p.grid_w % 4 == 0;
         const int table_n = grid ? P.table_st * (2 * p.reach_y + 1) : 0;
         float *const table = (float *)(sm + C::MORE + P.words * 32) + q * (table_n + 3) / 4 * 4;
         int *const places = (int *)((float *)(sm + C::MORE + P.words * 32) + 2 * ((table_n + 3) / 4 * 4));
@@ -544,7 +573,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             named_bar_sync(3, 256);
         }
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t s_phase = 0, o_phase = 0, p_phase = 0;
+        bool p_made = false;  // probabilities were handed on before
         for (; walk.next(P, x); turn++) {
             if (grid && table_h != x.h) {
                 // (a warp whose wait gave up still comes to these barriers)
@@ -590,23 +620,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                 for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, s + 32 * c);
                 tmem_wait_ld();
-                if (P.scaled) {
-                    if (p.cap_out > 0.f) {
+                if (C::APART) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty + 8 * q);
+                }
+                if (scaled) {
+                    if (capped) {
 #pragma unroll
                         for (int c = 0; c < 128; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
-                    } else if (!grid) {
+                    } else if (FORM != kFormGrid && !(FORM == kFormAny && grid)) {
 #pragma unroll
                         for (int c = 0; c < 128; c++) s[c] *= p.scale;
                     }
-                    if (P.bias_form == kBiasSlope) {
+                    if (FORM == kFormSlope || (FORM == kFormAny && P.bias_form == kBiasSlope)) {
                         const float d0 = (float)(r.at - j0);
 #pragma unroll
                         for (int c = 0; c < 128; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
-                    } else if (P.bias_form == kBiasLine) {
+                    } else if (FORM == kFormAny && P.bias_form == kBiasLine) {
 #pragma unroll
                         for (int c = 0; c < 128; c++) s[c] += table_bias(p, r, 0, j0 + c);
                     } else if (grid) {
-                        const float f = p.cap_out > 0.f ? 1.f : p.scale;
+                        const float f = capped ? 1.f : p.scale;
                         const F2 ff = f2(f, f);
                         if (quads) {
 #pragma unroll
@@ -664,6 +699,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     top[y] = fmaxf(top[y], s[124 + y]);
                 }
                 const float now = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+                if (C::APART && p_made) {
+                    // the product before is done with the probabilities and the outputs
+                    if (!(ok = mbar_wait_warp(p_empty + 8 * q, p_phase, P.err, 216))) break;
+                    p_phase ^= 1;
+                    tc_fence_after();
+                }
+                p_made = true;
                 // (m is -inf until a row has seen a key)
                 if (__any_sync(0xffffffffu, now * sc > m * sc + 8.f || (m == -INFINITY && now > m))) {
                     const float to = fmaxf(m, now), alpha = exp2_fast((m - (to == -INFINITY ? 0.f : to)) * sc);
@@ -698,7 +740,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         sum[y & 1] = f2_add(sum[y & 1], f2(a, z));
                         w[y] = MmaOp<T>::pack(a, z);
                     }
-                    tmem_st16(s_at + 16 * c, w);
+                    tmem_st16(p_at + 16 * c, w);
                 }
                 float la, lb;
                 f2_out(f2_add(sum[0], sum[1]), la, lb);
