@@ -3,7 +3,8 @@
  *
  * A block takes 256 queries of one head as two tiles of 128 and walks the keys in tiles of 128.
  * Warps 0-3 and 4-7 do the softmax of one query tile each (a thread a row), warp 8 issues the TMA
- * copies, warp 9 the matrix products, warps 10 and 11 look up which key tiles hold which documents:
+ * copies, warps 9 and 10 the products of a query tile each (one warp for both waited for one tile's
+ * softmax with the other's ready), warp 11 looks up which key tiles hold which documents:
  *   S_q = Q_q K^T   (both from shared memory)       -> TMEM, 128 columns each
  *   O_q += P_q V    (P from TMEM, V from shared)    -> TMEM, DP columns each
  * At 128 components P_q takes the columns of S_q (a thread holds its whole row of scores in registers
@@ -56,7 +57,7 @@ template <int DP> struct TcCfg {
     static constexpr int TILE = 128 * DP * 2;          // a tile of queries, keys or values
     static constexpr int Q = 0, K = 2 * TILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
     static constexpr int BARS = SCRATCH + 8 * 256 * 4;  // attend_row's queries, a warp each
-    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 4;
+    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 4 + 8 + 2;
     // With up to 64 components TMEM has room for probabilities beside the scores (P at 256 + 64 q, O at
     // 384 + 64 q): the next scores are computed as soon as the last are in registers.
     static constexpr bool APART = DP == 64;
@@ -97,6 +98,30 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(int N, boo
     const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (type << 7) | (type << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
+}
+// mbar_wait with a hint (10 us) of how long the hardware may keep a waiting thread asleep: the roles of
+// this kernel wait for one another most of the time, and polling took their issue slots.
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err, int code)
+{
+    if (mbar_test_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer();
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(10000u)
+            : "memory");
+        if (done) return true;
+        if (globaltimer() - t0 > 2000000000ull) {
+            atomicCAS(err, 0, code);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool tc_wait_warp(uint32_t bar, uint32_t parity, int *err, int code)
+{
+    return __all_sync(0xffffffffu, tc_wait(bar, parity, err, code));
 }
 // One lane of a converged warp. (Told by a lane number instead, the compiler takes the operands of the
 // branch's products and copies for divergent, and each issue costs 140 cycles instead of a few.)
@@ -163,6 +188,35 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// 2^x of two, on the FMA pipe: x = i + f with i whole and f in [-1/2, 1/2] (adding 1.5 * 2^23 rounds x to
+// i in the low bits), 2^f by a polynomial (minimax fit of degree 4, relative error 2.7e-6: 1/180 of
+// fp16's half step, to which the result is rounded), times 2^i; 0 below 2^-126.5 (i = -127 has no bits left), -inf included. NaN stays NaN.
+__device__ __forceinline__ F2 f2_exp2(float a, float b)
+{
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+    const F2 x = f2(a, b), magic = f2(12582912.f, 12582912.f);
+    const F2 r = f2_add(x, magic), f = f2_add(x, f2_fma(r, f2(-1.f, -1.f), magic));
+    F2 y = f2_fma(f2(0.009567738510668278f, 0.009567738510668278f), f, f2(0.05591749772429466f, 0.05591749772429466f));
+    y = f2_fma(y, f, f2(0.24024811387062073f, 0.24024811387062073f));
+    y = f2_fma(y, f, f2(0.6931219100952148f, 0.6931219100952148f));
+    y = f2_fma(y, f, f2(0.9999992251396179f, 0.9999992251396179f));
+    float ra, rb;
+    f2_out(r, ra, rb);
+    return f2_mul(y, f2(__int_as_float((__float_as_int(ra) << 23) + 0x3f800000), __int_as_float((__float_as_int(rb) << 23) + 0x3f800000)));
+}
+// tanh of two in [-1, 1] on the FMA pipe: odd polynomial of degree 11 (minimax fit, error 3e-7).
+__device__ __forceinline__ F2 f2_tanh(F2 x)
+{
+    const F2 z = f2_mul(x, x);
+    F2 y = f2_fma(f2(-0.0028189276345074177f, -0.0028189276345074177f), z, f2(0.01605205424129963f, 0.01605205424129963f));
+    y = f2_fma(y, z, f2(-0.050903141498565674f, -0.050903141498565674f));
+    y = f2_fma(y, z, f2(0.1325000524520874f, 0.1325000524520874f));
+    y = f2_fma(y, z, f2(-0.33323246240615845f, -0.33323246240615845f));
+    y = f2_fma(y, z, f2(0.9999963641166687f, 0.9999963641166687f));
+    return f2_mul(y, x);
 }
 
 // The lowest n bits of a word, n of any sign or size.
@@ -282,7 +336,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * C::ST,
                    v_full = k_empty + 8 * C::ST, v_empty = v_full + 8 * C::ST, s_full = v_empty + 8 * C::ST,
                    s_empty = s_full + 16, p_full = s_empty + 16, p_empty = p_full + 16, o_full = p_empty + 16,
-                   bits_full = o_full + 16, bits_empty = bits_full + 16;
+                   bits_full = o_full + 16, bits_empty = bits_full + 16, go = bits_empty + 16,
+                   p_half = go + 64;
     uint32_t *const tmem_at = (uint32_t *)(sm + C::BARS + C::NBAR * 8);
     uint32_t *const bit_sets = (uint32_t *)(sm + C::MORE);
 
@@ -292,8 +347,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tma_prefetch_desc(&mq);
         tma_prefetch_desc(&mk);
         tma_prefetch_desc(&mv);
-        for (uint32_t x = bars; x < bits_empty + 16; x += 8)
-            mbar_init(x, x >= bits_empty ? 10 : x >= bits_full ? 2 : x >= s_empty && x < p_empty ? 4 : 1);
+        for (uint32_t x = bars; x < p_half + 16; x += 8)
+            mbar_init(x, x >= p_half ? 4 : x >= go ? 1 : x >= bits_empty ? 11 : x >= s_empty && x < p_empty ? 4 : x >= k_empty && x < v_full || x >= v_empty && x < s_full ? 2 : 1);
         fence_mbar_init();
     }
     tc_fence_before();
@@ -319,11 +374,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 bool v_here = true;  // whether the last keys' values were asked for as well
                 for (; ok && walk.next(P, x); turn++) {
                     const uint32_t *bits = bits_of(turn);
-                    if (bits && !(ok = mbar_wait(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
+                    if (bits && !(ok = tc_wait(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
                     const int g = x.h / p.group;
                     bool q_here[2] = {false, false};
                     auto queries = [&](int q) {
-                        if (q_here[q] || !(ok = mbar_wait(q_empty + 8 * q, (nq[q] & 1) ^ 1, P.err, 200))) return;
+                        if (q_here[q] || !(ok = tc_wait(q_empty + 8 * q, (nq[q] & 1) ^ 1, P.err, 200))) return;
                         mbar_arrive_expect_tx(q_full + 8 * q, C::TILE);
                         for (int y = 0; y < DP / 64; y++)
                             tma_load_4d(s0 + C::Q + q * C::TILE + y * 16384, &mq, q_full + 8 * q, 64 * y, x.row0 + 128 * q, x.h,
@@ -337,14 +392,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const int st = n % C::ST;
                         const uint32_t parity = ((n / C::ST) & 1) ^ 1;
                         if (act[0]) queries(0);
-                        if (!ok || !(ok = mbar_wait(k_empty + 8 * st, parity, P.err, 201))) break;
+                        if (!ok || !(ok = tc_wait(k_empty + 8 * st, parity, P.err, 201))) break;
                         mbar_arrive_expect_tx(k_full + 8 * st, C::TILE);
                         for (int y = 0; y < DP / 64; y++)
                             tma_load_4d(s0 + C::K + st * C::TILE + y * 16384, &mk, k_full + 8 * st, 64 * y, t * kTcKeys, g, x.b);
                         n++;
                         v_here = false;
                         if (act[1]) queries(1);
-                        if (!ok || !(ok = mbar_wait(v_empty + 8 * st, parity, P.err, 202))) break;
+                        if (!ok || !(ok = tc_wait(v_empty + 8 * st, parity, P.err, 202))) break;
                         mbar_arrive_expect_tx(v_full + 8 * st, C::TILE);
                         for (int y = 0; y < DP / 64; y++)
                             tma_load_4d(s0 + C::V + st * C::TILE + y * 16384, &mv, v_full + 8 * st, 64 * y, t * kTcKeys, g, x.b);
@@ -355,139 +410,132 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // every copy has landed before the block ends, also where a wait gave up
 #pragma unroll
                 for (int q = 0; q < 2; q++)
-                    if (nq[q]) mbar_wait(q_full + 8 * q, (nq[q] - 1) & 1, P.err, 203);
+                    if (nq[q]) tc_wait(q_full + 8 * q, (nq[q] - 1) & 1, P.err, 203);
                 for (int i = max(0, n - C::ST); i < n; i++) {
-                    mbar_wait(k_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 204);
-                    if (v_here || i < n - 1) mbar_wait(v_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 205);
+                    tc_wait(k_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 204);
+                    if (v_here || i < n - 1) tc_wait(v_full + 8 * (i % C::ST), (i / C::ST) & 1, P.err, 205);
                 }
             }
-        } else if (warp == 9) {
-            // ---- products ----
+        } else if (warp < 11) {
+            // ---- products of query tile q ----
+            const int q = warp - 9;
             // N of P V: the components, in sixteens; k of Q K^T likewise
             const int dn = (p.d + 15) / 16 * 16;
             const uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(dn, true);
-            uint32_t phase = 0;  // of p_full (bits 0, 1), q_full (2, 3) and s_empty (4, 5)
+            const uint32_t s_at = tmem + 128 * q, p_at = tmem + C::P_AT + C::P_Q * q, o_at = tmem + C::O_AT + C::O_Q * q;
+            const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::TILE, 16);
+            uint32_t phase = 0;  // of p_full (bit 0), q_full (1), s_empty (2) and p_half (3)
             auto wait = [&](uint32_t bar, int bit, int code) {
-                const bool done = mbar_wait_warp(bar, phase >> bit & 1, P.err, code);
+                const bool done = tc_wait_warp(bar + 8 * q, phase >> bit & 1, P.err, code);
                 phase ^= 1u << bit;
                 return done;
             };
-            int n = 0;
-            uint32_t s_made = 0;  // scores computed before, by query tile: their columns are to be free again
+            int n = 0;            // key tiles so far, of both query tiles
+            bool made = false;    // scores were computed before: their columns are to be free again
             for (; ok && walk.next(P, x); turn++) {
                 const uint32_t *bits = bits_of(turn);
-                if (bits && !(ok = mbar_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
-                uint32_t pend = 0, acc = 0, q_here = 0;  // by query tile
-                int t_prev = 0;
-                bool prev = false;  // a key tile of this item has gone before
-                // S_q = Q_q K^T of key tile t, the n-th
-                auto scores = [&](int q, bool &k_here) {
-                    const int st = n % C::ST;
-                    if (!(q_here >> q & 1)) {
-                        if (!wait(q_full + 8 * q, 2 + q, 209)) return false;
-                        q_here |= 1u << q;
-                    }
-                    if (!k_here && !mbar_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208)) return false;
-                    k_here = true;
-                    if (C::APART) {
-                        if (s_made >> q & 1) {
-                            if (!wait(s_empty + 8 * q, 4 + q, 215)) return false;
-                            tc_fence_after();
+                if (bits && !(ok = tc_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
+                bool q_here = false, acc = false;
+                int n_pend = -1, t_pend = 0;  // the key tile whose scores the softmax warps have
+                // O += P V of that key tile
+                auto values = [&]() {
+                    const int st = n_pend % C::ST;
+                    if (!tc_wait_warp(v_full + 8 * st, (n_pend / C::ST) & 1, P.err, 206)) return false;
+                    const int live = x.kn - t_pend * kTcKeys;
+                    if (live < kTcKeys && x.kn < p.lk) {
+                        // values behind the last key may be anything: zeros (from both warps), as 0 * NaN is NaN
+                        for (int i = lane; i < (kTcKeys - live) * (DP / 8); i += 32) {
+                            const int r = live + i / (DP / 8), c = i % (DP / 8);
+                            *reinterpret_cast<uint4 *>(sm + C::V + st * C::TILE + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
                         }
-                        s_made |= 1u << q;
+                        fence_proxy_async();
+                        __syncwarp();
                     }
-                    if (elect_one()) {
-                        const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::TILE, 16), kd = swizzled_desc(s0 + C::K + st * C::TILE, 16);
-#pragma unroll
-                        for (int kk = 0; kk < DP / 16; kk++) {
-                            const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-                            if (kk * 16 < p.d) mma_f16(tmem + 128 * q, qd + at, kd + at, id_s, kk > 0, 0);
-                        }
-                        mma_commit(s_full + 8 * q);
-                    }
-                    return true;
-                };
-                // O_q += P_q V of the key tile before
-                auto values = [&](int q, bool &v_here) {
-                    const int st = (n - 1) % C::ST;
-                    const uint32_t vs = s0 + C::V + st * C::TILE;
-                    if (!v_here) {
-                        if (!mbar_wait_warp(v_full + 8 * st, ((n - 1) / C::ST) & 1, P.err, 206)) return false;
-                        const int live = x.kn - t_prev * kTcKeys;
-                        if (live < kTcKeys && x.kn < p.lk) {
-                            // values behind the last key may be anything: zeros, as 0 * NaN is NaN
-                            for (int i = lane; i < (kTcKeys - live) * (DP / 8); i += 32) {
-                                const int r = live + i / (DP / 8), c = i % (DP / 8);
-                                *reinterpret_cast<uint4 *>(sm + C::V + st * C::TILE + (c >> 3) * 16384 + r * 128 +
-                                                           (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async();
-                            __syncwarp();
-                        }
-                        v_here = true;
-                    }
-                    if (!wait(p_full + 8 * q, q, 207)) return false;
+                    const uint64_t vd = swizzled_desc(s0 + C::V + st * C::TILE, 16384);
+                    if (!wait(p_half, 3, 218)) return false;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t vd = swizzled_desc(vs, 16384);
 #pragma unroll
-                        for (int kk = 0; kk < kTcKeys / 16; kk++)
-                            mma_f16_ts(tmem + C::O_AT + C::O_Q * q, tmem + C::P_AT + C::P_Q * q + 8 * kk, vd + (kk * 2048 >> 4), id_o,
-                                       (acc >> q & 1) || kk > 0);
-                        if (C::APART) mma_commit(p_empty + 8 * q);
+                        for (int kk = 0; kk < kTcKeys / 32; kk++)
+                            mma_f16_ts(o_at, p_at + 8 * kk, vd + (kk * 2048 >> 4), id_o, acc || kk > 0);
                     }
-                    acc |= 1u << q;
+                    __syncwarp();
+                    if (!wait(p_full, 0, 207)) return false;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = kTcKeys / 32; kk < kTcKeys / 16; kk++)
+                            mma_f16_ts(o_at, p_at + 8 * kk, vd + (kk * 2048 >> 4), id_o, 1u);
+                        if (C::APART) mma_commit(p_empty + 8 * q);
+                        mma_commit(v_empty + 8 * st);
+                    }
+                    __syncwarp();
+                    acc = true;
+                    n_pend = -1;
                     return true;
                 };
                 for (int t = x.t0; t < x.t1 && ok; t++) {
-                    const bool a0 = tc_active(x, bits, 0, t), a1 = tc_active(x, bits, 1, t);
-                    if (!a0 && !a1) continue;
-                    bool v_here = false, k_here = false;
-                    if (C::APART) {
-                        ok = (!a0 || scores(0, k_here)) && (!a1 || scores(1, k_here)) && (!(pend & 1) || values(0, v_here)) &&
-                             (!(pend & 2) || values(1, v_here));
+                    const bool mine = tc_active(x, bits, q, t);
+                    if (!mine && !tc_active(x, bits, 1 - q, t)) continue;
+                    const int st = n % C::ST;
+                    if (mine) {
+                        // the scores' columns: free once the product with the values that reads them is issued, or (APART)
+                        // once they are in registers
+                        if (!C::APART && n_pend >= 0 && !(ok = values())) break;
+                        if (!q_here && !(ok = wait(q_full, 1, 209))) break;
+                        q_here = true;
+                        if (!(ok = tc_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208))) break;
+                        if (C::APART && made) {
+                            if (!(ok = wait(s_empty, 2, 215))) break;
+                            tc_fence_after();
+                        }
+                        made = true;
+                        if (elect_one()) {
+                            const uint64_t kd = swizzled_desc(s0 + C::K + st * C::TILE, 16);
+#pragma unroll
+                            for (int kk = 0; kk < DP / 16; kk++) {
+                                const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+                                if (kk * 16 < p.d) mma_f16(s_at, qd + at, kd + at, id_s, kk > 0, 0);
+                            }
+                            mma_commit(s_full + 8 * q);
+                            mma_commit(k_empty + 8 * st);
+                        }
+                        __syncwarp();
+                        if (C::APART && n_pend >= 0 && !(ok = values())) break;
+                        n_pend = n;
+                        t_pend = t;
                     } else {
-                        ok = (!(pend & 1) || values(0, v_here)) && (!a0 || scores(0, k_here)) &&
-                             (!(pend & 2) || values(1, v_here)) && (!a1 || scores(1, k_here));
+                        // the other query tile's alone; this one's last is not held back behind it
+                        if (n_pend >= 0 && !(ok = values())) break;
+                        // (not ahead of the copies: an arrival a stage and turn)
+                        if (!(ok = tc_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208))) break;
+                        if (!(ok = tc_wait_warp(v_full + 8 * st, (n / C::ST) & 1, P.err, 206))) break;
+                        if (lane == 0) {
+                            mbar_arrive(k_empty + 8 * st);
+                            mbar_arrive(v_empty + 8 * st);
+                        }
+                        __syncwarp();
                     }
-                    pend = (a0 ? 1u : 0u) | (a1 ? 2u : 0u);
-                    if (ok && elect_one()) {
-                        mma_commit(k_empty + 8 * (n % C::ST));
-                        if (prev) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
-                    }
-                    __syncwarp();
-                    t_prev = t;
-                    prev = true;
                     n++;
                 }
-                // the queries are free when the last scores are there; the outputs of each tile as it ends
-                if (ok && elect_one()) {
-                    if (q_here & 1) mma_commit(q_empty);
-                    if (q_here & 2) mma_commit(q_empty + 8);
-                }
-                bool v_here = false;
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    if (ok && (pend >> q & 1)) ok = values(q, v_here);
-                    if (ok && (acc >> q & 1) && elect_one()) mma_commit(o_full + 8 * q);
-                }
-                if (ok && prev && elect_one()) mma_commit(v_empty + 8 * ((n - 1) % C::ST));
+                // the queries are free when the last scores are there
+                if (ok && q_here && elect_one()) mma_commit(q_empty + 8 * q);
+                if (ok && n_pend >= 0) ok = values();
+                if (ok && acc && elect_one()) mma_commit(o_full + 8 * q);
                 if (bits && lane == 0) mbar_arrive(bits_empty + 8 * (turn & 1));
                 __syncwarp();
             }
             // no product is in flight when the block ends (the softmax warps do not wait where a wait gave up)
             if (!ok) {
-                if (elect_one()) {
-                    mma_commit(o_full);
-                    mma_commit(o_full + 8);
-                }
+                if (elect_one()) mma_commit(o_full + 8 * q);
                 __syncwarp();
-                for (int i = 0; i < 2; i++) mbar_wait_warp(o_full, i, P.err, 212);
+                for (int i = 0; i < 2; i++) tc_wait_warp(o_full + 8 * q, i, P.err, 212);
             }
         } else if (documents) {
             // ---- documents: which key tiles hold one of a query tile's, and which nothing but its only one ----
             for (; ok && walk.next(P, x); turn++) {
-                if (!(ok = mbar_wait_warp(bits_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214))) break;
+                if (!(ok = tc_wait_warp(bits_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214))) break;
                 uint32_t *bits = bit_sets + (turn & 1) * P.words * 4;
                 const int *qd = p.q_doc + (int64_t)(x.b % p.doc_rows) * p.lq, *kd = p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk;
                 int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
@@ -506,7 +554,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
                 }
                 const int word0 = x.t0 / 32;
-                for (int w = word0 + warp - 10; w * 32 < x.t1; w += 2) {
+                for (int w = word0; w * 32 < x.t1; w++) {
                     int klo = INT_MAX, khi = INT_MIN;
                     for (int y = max(x.t0 - w * 32, 0); y < min(x.t1 - w * 32, 32); y += 4) {
                         // four tiles' loads in flight; lane l keeps tile l's range
@@ -573,8 +621,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             named_bar_sync(3, 256);
         }
+        constexpr int CH = 32;
         uint32_t s_phase = 0, o_phase = 0, p_phase = 0;
         bool p_made = false;  // probabilities were handed on before
+        // Warps w and w + 4 share a scheduler and its exponential unit (4 a cycle): they take turns, so that
+        // one's exponentials run beside the other's products, loads and maxima and not beside its exponentials.
+        uint32_t turns = q ? 0 : 1;
+        auto my_turn = [&]() {
+            const bool done = tc_wait_warp(go + 8 * warp, turns & 1, P.err, 217);
+            turns++;
+            return done;
+        };
+        auto pass_turn = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(go + 8 * (warp ^ 4));
+        };
         for (; walk.next(P, x); turn++) {
             if (grid && table_h != x.h) {
                 // (a warp whose wait gave up still comes to these barriers)
@@ -589,7 +650,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             if (!ok) continue;
             const uint32_t *bits = bits_of(turn);
-            if (bits && !(ok = mbar_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) continue;
+            if (bits && !(ok = tc_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) continue;
             const int i = x.row0 + 128 * q + r_in;
             const bool there = i < x.qn;
             const Query r = query_of(p, x.b, x.h, min(i, x.qn - 1), x.qn, x.kn);
@@ -600,108 +661,139 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float m = -INFINITY, l = 0.f;  // m: in the units of the scores; times sc it is base 2
             bool any = false;
             for (int t = x.t0; t < x.t1; t++) {
-                if (!(t < before || (t >= from && t < to))) continue;
+                bool seen_here = t < before || (t >= from && t < to);
                 bool all = t < x.full && (t < x.before_whole || (t >= whole_from && t < whole_to));
                 if (bits) {
-                    const uint32_t *word = bits + 4 * (t / 32 - x.t0 / 32) + q;
-                    if (!(word[0] >> (t & 31) & 1)) continue;
-                    all = all && word[2] >> (t & 31) & 1;
+                    const uint32_t word = bits[4 * (t / 32 - x.t0 / 32) + q], whole = bits[4 * (t / 32 - x.t0 / 32) + 2 + q];
+                    seen_here = seen_here && (word >> (t & 31) & 1);
+                    all = all && (whole >> (t & 31) & 1);
+                }
+                if (!seen_here) {
+                    // the other query tile's alone: pass its turn on
+                    if (x.both && tc_active(x, bits, 1 - q, t)) {
+                        if (!(ok = my_turn())) break;
+                        pass_turn();
+                    }
+                    continue;
                 }
                 const int j0 = t * kTcKeys;
-                int ids[4];
-                if (docs && !all) {
-#pragma unroll
-                    for (int w = 0; w < 4; w++) ids[w] = __ldg(docs + min(j0 + 32 * w + lane, x.kn - 1));
-                }
-                if (!(ok = mbar_wait_warp(s_full + 8 * q, s_phase, P.err, 210))) break;
+                if (!(ok = tc_wait_warp(s_full + 8 * q, s_phase, P.err, 210))) break;
                 s_phase ^= 1;
                 tc_fence_after();
-                float s[128];
+                // Scores that are more than a scaled product are made in a first pass, CH columns at a time (a short
+                // loop: unrolled over the row its instructions are fetched anew every time), and put back.
+                if (scaled || !all) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < kTcKeys; c0 += CH) {
+                    float s[CH];
 #pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, s + 32 * c);
+                    for (int c = 0; c < CH; c += 32) tmem_ld32(s_at + c0 + c, s + c);
+                    tmem_wait_ld();
+                    if (scaled) {
+                        if (capped) {
+                            // exponentials and reciprocals of the tanh are three times the unit's work: below the cap a
+                            // polynomial does
+                            float far = 0.f;
+#pragma unroll
+                            for (int c = 0; c < CH; c += 2) far = max3(far, fabsf(s[c]), fabsf(s[c + 1]));
+                            if (__all_sync(0xffffffffu, far * fabsf(p.cap_in) <= 1.f)) {
+                                const F2 in = f2(p.cap_in, p.cap_in), out = f2(p.cap_out, p.cap_out);
+#pragma unroll
+                                for (int c = 0; c < CH; c += 2)
+                                    f2_out(f2_mul(f2_tanh(f2_mul(f2(s[c], s[c + 1]), in)), out), s[c], s[c + 1]);
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < CH; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
+                            }
+                        } else if (FORM != kFormGrid && !(FORM == kFormAny && grid)) {
+#pragma unroll
+                            for (int c = 0; c < CH; c++) s[c] *= p.scale;
+                        }
+                        if (FORM == kFormSlope || (FORM == kFormAny && P.bias_form == kBiasSlope)) {
+                            const float d0 = (float)(r.at - j0 - c0);
+#pragma unroll
+                            for (int c = 0; c < CH; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
+                        } else if (FORM == kFormAny && P.bias_form == kBiasLine) {
+#pragma unroll
+                            for (int c = 0; c < CH; c++) s[c] += table_bias(p, r, 0, j0 + c0 + c);
+                        } else if (grid) {
+                            const float f = capped ? 1.f : p.scale;
+                            const F2 ff = f2(f, f);
+                            if (quads) {
+#pragma unroll
+                                for (int c = 0; c < CH; c += 16) {
+                                    const int4 at = *reinterpret_cast<const int4 *>(places + ((j0 + c0 + c) >> 2));
+#pragma unroll
+                                    for (int y = 0; y < 16; y += 2) {
+                                        const float *e = mine + (y < 4 ? at.x : y < 8 ? at.y : y < 12 ? at.z : at.w) + (y & 3);
+                                        f2_out(f2_fma(f2(s[c + y], s[c + y + 1]), ff, f2(e[0], e[1])), s[c + y], s[c + y + 1]);
+                                    }
+                                }
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < CH; c += 4) {
+                                    const int4 at = *reinterpret_cast<const int4 *>(places + j0 + c0 + c);
+                                    s[c] = fmaf(s[c], f, mine[at.x]);
+                                    s[c + 1] = fmaf(s[c + 1], f, mine[at.y]);
+                                    s[c + 2] = fmaf(s[c + 2], f, mine[at.z]);
+                                    s[c + 3] = fmaf(s[c + 3], f, mine[at.w]);
+                                }
+                            }
+                        }
+                    }
+                    if (!all) {
+#pragma unroll
+                        for (int w = 0; w < CH; w += 32) {
+                            // a bit a key: [0, below) or [lo, hi), below end, of this query's document
+                            const int j = j0 + c0 + w, lo = max(r.lo, 0) - j, hi = min(r.hi == INT_MAX ? INT_MAX : r.hi - j, 31) + 1;
+                            uint32_t seen = ((bits_below(hi) & ~bits_below(lo)) | bits_below(r.pre - j)) & bits_below(x.kn - j);
+                            if (docs) {
+                                // one vote for each document among the warp's queries
+                                const int key = __ldg(docs + min(j + lane, x.kn - 1));
+                                for (uint32_t left = 0xffffffffu; left;) {
+                                    const int id = __shfl_sync(0xffffffffu, r.doc, __ffs(left) - 1);
+                                    const bool same = r.doc == id;
+                                    const uint32_t of = __ballot_sync(0xffffffffu, key == id);
+                                    if (same) seen &= of;
+                                    left &= ~__ballot_sync(0xffffffffu, same);
+                                }
+                            }
+#pragma unroll
+                            for (int c = 0; c < 32; c++) s[w + c] = seen >> c & 1 ? s[w + c] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < CH; c += 16) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int y = 0; y < 16; y++) w[y] = __float_as_uint(s[c + y]);
+                        tmem_st16(s_at + c0 + c, w);
+                    }
+                }
+                tmem_wait_st();
+                }
+                float s[kTcKeys];
+#pragma unroll
+                for (int c = 0; c < kTcKeys; c += 32) tmem_ld32(s_at + c, s + c);
                 tmem_wait_ld();
                 if (C::APART) {
+                    // the scores are in registers: their columns are free
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s_empty + 8 * q);
-                }
-                if (scaled) {
-                    if (capped) {
-#pragma unroll
-                        for (int c = 0; c < 128; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
-                    } else if (FORM != kFormGrid && !(FORM == kFormAny && grid)) {
-#pragma unroll
-                        for (int c = 0; c < 128; c++) s[c] *= p.scale;
-                    }
-                    if (FORM == kFormSlope || (FORM == kFormAny && P.bias_form == kBiasSlope)) {
-                        const float d0 = (float)(r.at - j0);
-#pragma unroll
-                        for (int c = 0; c < 128; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
-                    } else if (FORM == kFormAny && P.bias_form == kBiasLine) {
-#pragma unroll
-                        for (int c = 0; c < 128; c++) s[c] += table_bias(p, r, 0, j0 + c);
-                    } else if (grid) {
-                        const float f = capped ? 1.f : p.scale;
-                        const F2 ff = f2(f, f);
-                        if (quads) {
-#pragma unroll
-                            for (int c = 0; c < 128; c += 16) {
-                                const int4 at = *reinterpret_cast<const int4 *>(places + ((j0 + c) >> 2));
-#pragma unroll
-                                for (int y = 0; y < 16; y += 2) {
-                                    const float *e = mine + (y < 4 ? at.x : y < 8 ? at.y : y < 12 ? at.z : at.w) + (y & 3);
-                                    f2_out(f2_fma(f2(s[c + y], s[c + y + 1]), ff, f2(e[0], e[1])), s[c + y], s[c + y + 1]);
-                                }
-                            }
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 128; c += 4) {
-                                const int4 at = *reinterpret_cast<const int4 *>(places + j0 + c);
-                                s[c] = fmaf(s[c], f, mine[at.x]);
-                                s[c + 1] = fmaf(s[c + 1], f, mine[at.y]);
-                                s[c + 2] = fmaf(s[c + 2], f, mine[at.z]);
-                                s[c + 3] = fmaf(s[c + 3], f, mine[at.w]);
-                            }
-                        }
-                    }
-                }
-                if (!all) {
-                    // a bit a key: [0, below) or [lo, hi), below end, of this query's document
-                    const int lo = max(r.lo, 0) - j0, hi = min(r.hi == INT_MAX ? INT_MAX : r.hi - j0, 127) + 1;
-                    const int below = min(r.pre - j0, 128), end = min(x.kn - j0, 128);
-                    uint32_t seen[4];
-#pragma unroll
-                    for (int w = 0; w < 4; w++)
-                        seen[w] = ((bits_below(hi - 32 * w) & ~bits_below(lo - 32 * w)) | bits_below(below - 32 * w)) &
-                                  bits_below(end - 32 * w);
-                    if (docs) {
-                        // one vote for each document among the warp's queries
-                        for (uint32_t left = 0xffffffffu; left;) {
-                            const int id = __shfl_sync(0xffffffffu, r.doc, __ffs(left) - 1);
-                            const bool same = r.doc == id;
-#pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                const uint32_t of = __ballot_sync(0xffffffffu, ids[w] == id);
-                                if (same) seen[w] &= of;
-                            }
-                            left &= ~__ballot_sync(0xffffffffu, same);
-                        }
-                    }
-#pragma unroll
-                    for (int c = 0; c < 128; c++) s[c] = seen[c >> 5] >> (c & 31) & 1 ? s[c] : -INFINITY;
                 }
                 float top[4];
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
                     top[y] = s[y];
 #pragma unroll
-                    for (int c = 4 + y; c < 124; c += 8) top[y] = max3(top[y], s[c], s[c + 4]);
-                    top[y] = fmaxf(top[y], s[124 + y]);
+                    for (int c = 4 + y; c < kTcKeys - 4; c += 8) top[y] = max3(top[y], s[c], s[c + 4]);
+                    top[y] = fmaxf(top[y], s[kTcKeys - 4 + y]);
                 }
                 const float now = max3(fmaxf(top[0], top[1]), top[2], top[3]);
                 if (C::APART && p_made) {
                     // the product before is done with the probabilities and the outputs
-                    if (!(ok = mbar_wait_warp(p_empty + 8 * q, p_phase, P.err, 216))) break;
+                    if (!(ok = tc_wait_warp(p_empty + 8 * q, p_phase, P.err, 216))) break;
                     p_phase ^= 1;
                     tc_fence_after();
                 }
@@ -710,15 +802,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (__any_sync(0xffffffffu, now * sc > m * sc + 8.f || (m == -INFINITY && now > m))) {
                     const float to = fmaxf(m, now), alpha = exp2_fast((m - (to == -INFINITY ? 0.f : to)) * sc);
                     if (any) {
-                        for (int c = 0; c < p.d; c += 32) {
-                            float o[32];
-                            tmem_ld32(o_at + c, o);
+#pragma unroll 1
+                        for (int c = 0; c < p.d; c += 16) {
+                            float o[16];
+                            tmem_ld16(o_at + c, o);
                             tmem_wait_ld();
-                            uint32_t w[2][16];
+                            uint32_t w[16];
 #pragma unroll
-                            for (int y = 0; y < 32; y++) w[y >> 4][y & 15] = __float_as_uint(o[y] * alpha);
-                            tmem_st16(o_at + c, w[0]);
-                            tmem_st16(o_at + c + 16, w[1]);
+                            for (int y = 0; y < 16; y++) w[y] = __float_as_uint(o[y] * alpha);
+                            tmem_st16(o_at + c, w);
                         }
                     }
                     l *= m == -INFINITY ? 0.f : alpha;
@@ -727,21 +819,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 any = true;
                 const float base = m == -INFINITY ? 0.f : m * sc;
                 const F2 sc2 = f2(sc, sc), base2 = f2(-base, -base);
+#pragma unroll
+                for (int c = 0; c < kTcKeys; c += 2) f2_out(f2_fma(f2(s[c], s[c + 1]), sc2, base2), s[c], s[c + 1]);
+                if (x.both && !(ok = my_turn())) break;
                 F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < kTcKeys; c += 32) {
                     uint32_t w[16];
 #pragma unroll
                     for (int y = 0; y < 16; y++) {
+                        F2 e;
+                        if (y % 4 == 3)  // a quarter of them on the FMA pipe
+                            e = f2_exp2(s[c + 2 * y], s[c + 2 * y + 1]);
+                        else
+                            e = f2(exp2_fast(s[c + 2 * y]), exp2_fast(s[c + 2 * y + 1]));
+                        sum[y & 1] = f2_add(sum[y & 1], e);
                         float a, z;
-                        f2_out(f2_fma(f2(s[32 * c + 2 * y], s[32 * c + 2 * y + 1]), sc2, base2), a, z);
-                        a = exp2_fast(a);
-                        z = exp2_fast(z);
-                        sum[y & 1] = f2_add(sum[y & 1], f2(a, z));
+                        f2_out(e, a, z);
                         w[y] = MmaOp<T>::pack(a, z);
                     }
-                    tmem_st16(p_at + 16 * c, w);
+                    tmem_st16(p_at + c / 2, w);
+                    if (c == kTcKeys / 2 - 32) {
+                        // the product with the first half of the values can start
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_half + 8 * q);
+                    }
                 }
+                if (x.both) pass_turn();
                 float la, lb;
                 f2_out(f2_add(sum[0], sum[1]), la, lb);
                 l += la + lb;
@@ -758,7 +864,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
             // ---- out: a thread a row ----
             if (any) {
-                if (!(ok = mbar_wait_warp(o_full + 8 * q, o_phase, P.err, 211))) continue;
+                if (!(ok = tc_wait_warp(o_full + 8 * q, o_phase, P.err, 211))) continue;
                 o_phase ^= 1;
                 tc_fence_after();
             }
