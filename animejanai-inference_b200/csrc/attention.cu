@@ -98,9 +98,9 @@ cudaError_t run(const MmaDev &p, const Choice &c, cudaStream_t s)
     return cudaGetLastError();
 }
 
-// A tensor map of 128-token tiles of 64 components of one head (128-byte swizzle; zeros outside).
+// A tensor map of tiles of `rows` tokens, 64 components of one head (128-byte swizzle; zeros outside).
 // False if the layout does not allow one (16-byte aligned, no repeated dimension).
-bool map_of(CUtensorMap *m, const ajib_heads *x, int batch, int tokens, int heads, int d, int dtype)
+bool map_of(CUtensorMap *m, const ajib_heads *x, int batch, int tokens, int heads, int d, int dtype, int rows)
 {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -121,7 +121,7 @@ bool map_of(CUtensorMap *m, const ajib_heads *x, int batch, int tokens, int head
         dims[i + 1] = (cuuint64_t)n[i];
         strides[i] = n[i] > 1 ? (cuuint64_t)st[i] * 2 : 16;  // (never used)
     }
-    const cuuint32_t box[4] = {64, 128, 1, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, one[4] = {1, 1, 1, 1};
     return encode(m, dtype == AJIB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x->p, dims,
                   strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -244,8 +244,9 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         m.bias_form = !op->grid_w ? kBiasLine : grid_reached(op) ? kBiasGridDirect : kBiasGrid;
     }
     CUtensorMap maps[3];
-    if (c.tc && map_of(&maps[0], q, b, op->lq, op->hq, d, op->dtype) && map_of(&maps[1], k, b, op->lk, op->hk, d, op->dtype) &&
-        map_of(&maps[2], v, b, op->lk, op->hk, d, op->dtype)) {
+    const int key_tile = d <= 64 ? TcCfg<64>::KT : TcCfg<128>::KT;
+    if (c.tc && map_of(&maps[0], q, b, op->lq, op->hq, d, op->dtype, 128) && map_of(&maps[1], k, b, op->lk, op->hk, d, op->dtype, key_tile) &&
+        map_of(&maps[2], v, b, op->lk, op->hk, d, op->dtype, key_tile)) {
         TcDev t{};
         t.a = p;
         t.tiles = (op->lq + 255) / 256;

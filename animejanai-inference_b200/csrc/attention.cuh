@@ -82,16 +82,16 @@ struct Query {
     const float *table;
 };
 
-__device__ __forceinline__ Query query_of(const AttnDev &p, int b, int h, int i, int qn, int kn)
+__device__ __forceinline__ Query query_at(const AttnDev &p, int doc_row, int h, int i, int shift, int pre)
 {
     Query r;
-    r.at = i + (p.align_end ? kn - qn : 0);
+    r.at = i + shift;
     r.lo = p.left == INT_MAX / 2 ? INT_MIN : r.at - p.left;
     r.hi = p.right == INT_MAX / 2 ? INT_MAX : r.at + p.right;
-    r.pre = p.prefix ? max(__ldg(p.prefix + b), 0) : 0;
+    r.pre = pre;
     r.doc = INT_MIN;
     if (p.q_doc) {
-        r.doc = i < p.lq ? __ldg(p.q_doc + (int64_t)(b % p.doc_rows) * p.lq + i) : -1;
+        r.doc = __ldg(p.q_doc + (int64_t)doc_row * p.lq + i);
         if (r.doc < 0) r.lo = INT_MAX, r.hi = -1, r.pre = 0;  // padding sees nothing
     }
     r.y = 0;
@@ -107,6 +107,11 @@ __device__ __forceinline__ Query query_of(const AttnDev &p, int b, int h, int i,
         r.table = p.bias_data + (int64_t)h * (2 * p.reach_y + 1) * (2 * p.reach_x + 1);
     }
     return r;
+}
+
+__device__ __forceinline__ Query query_of(const AttnDev &p, int b, int h, int i, int qn, int kn)
+{
+    return query_at(p, p.q_doc ? b % p.doc_rows : 0, h, i, p.align_end ? kn - qn : 0, p.prefix ? max(__ldg(p.prefix + b), 0) : 0);
 }
 
 __device__ __forceinline__ bool in_reach(const Query &r, int j) { return j < r.pre || (j >= r.lo && j <= r.hi); }

@@ -33,7 +33,7 @@
 
 namespace ajib {
 
-constexpr int kTcThreads = 384, kTcKeys = 128;
+constexpr int kTcThreads = 384;
 
 // What happens to scores beside the scale; a kernel each, as code that is jumped over costs
 // instruction fetches. kFormAny looks at the op for everything.
@@ -53,19 +53,21 @@ struct TcDev {
 };
 
 template <int DP> struct TcCfg {
-    static constexpr int ST = DP == 128 ? 2 : 4;       // stages of keys and of values
-    static constexpr int TILE = 128 * DP * 2;          // a tile of queries, keys or values
-    static constexpr int Q = 0, K = 2 * TILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
+    static constexpr int KT = DP;                      // keys of a tile
+    static constexpr int BLOCKS = DP == 64 ? 2 : 1;    // on an SM
+    static constexpr int ST = DP == 64 ? 3 : 2;        // stages of keys and of values
+    static constexpr int QTILE = 128 * DP * 2, TILE = KT * DP * 2, HALF = KT * 128;  // HALF: a tile's 64 components
+    static constexpr int Q = 0, K = 2 * QTILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
     static constexpr int BARS = SCRATCH + 8 * 256 * 4;  // attend_row's queries, a warp each
-    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 4 + 8 + 2;
-    // With up to 64 components TMEM has room for probabilities beside the scores (P at 256 + 64 q, O at
-    // 384 + 64 q): the next scores are computed as soon as the last are in registers.
-    static constexpr bool APART = DP == 64;
-    static constexpr int P_AT = APART ? 256 : 0, P_Q = APART ? 64 : 128, O_AT = APART ? 384 : 256, O_Q = APART ? 64 : 128;
-    static constexpr int MORE = BARS + NBAR * 8 + 16;
+    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 8 + 4;
+    static constexpr int COLUMNS = 2 * KT + 2 * DP;     // of TMEM: scores of both query tiles, then outputs
+    // One block of 384 threads an SM: 168 registers, of which the softmax warps take 216 and the others 72.
+    // Two blocks: 80 each.
+    static constexpr int REGS = 216, REGS_REST = 72;
+    static constexpr int ITEMS = (BARS + NBAR * 8 + 31) / 16 * 16, MORE = ITEMS + 2 * 128;
     // behind: the bit sets (two, four words each for every 32 key tiles: seen and whole, of both query
     // tiles), or the table (one a softmax warpgroup) and its keys' places
-    static int bit_words(const ajib_attn *op) { return op->q_doc ? (op->lk + kTcKeys * 32 - 1) / (kTcKeys * 32) : 0; }
+    static int bit_words(const ajib_attn *op) { return op->q_doc ? (op->lk + KT * 32 - 1) / (KT * 32) : 0; }
     // Rows of the table start table_stride apart, so that the 32 queries of a warp, neighbours on the
     // grid, read 32 different banks.
     static int table_stride(const ajib_attn *op)
@@ -77,7 +79,7 @@ template <int DP> struct TcCfg {
     {
         int64_t n = MORE + 1024 + (int64_t)bit_words(op) * 32;  // 1024: the alignment of the first tile
         if (op->bias == AJIB_BIAS_TABLE && op->grid_w)
-            n += 2 * ((int64_t)table_stride(op) * (2 * op->reach_y + 1) * 4 + 16) + ((op->lk + 127) / 128 * 128) * 4;
+            n += 2 * ((int64_t)table_stride(op) * (2 * op->reach_y + 1) * 4 + 16) + ((op->lk + KT - 1) / KT * KT) * 4;
         return n;
     }
 };
@@ -219,13 +221,28 @@ __device__ __forceinline__ F2 f2_tanh(F2 x)
     return f2_mul(y, x);
 }
 
+template <int N> __device__ __forceinline__ float row_max(const float *s)
+{
+    float top[4];
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+        top[y] = s[y];
+#pragma unroll
+        for (int c = 4 + y; c < N - 4; c += 8) top[y] = max3(top[y], s[c], s[c + 4]);
+        top[y] = fmaxf(top[y], s[N - 4 + y]);
+    }
+    return max3(fmaxf(top[0], top[1]), top[2], top[3]);
+}
+
 // The lowest n bits of a word, n of any sign or size.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
 
-// One item's queries and keys, worked out alike by every role.
-struct TcItem {
-    int b, h, row0, qn, kn;
-    bool both;                 // there are queries in the second tile
+// One item's queries and keys, worked out by one warp for all of them.
+struct __align__(16) TcItem {
+    int b, h, row0, qn, kn;    // b < 0: no more items
+    int shift, pre;            // query i stands at i + shift; keys below pre are seen by all
+    int doc_row;
+    int both;                  // there are queries in the second tile
     int t0, t1;                // key tiles that any query sees
     int before, before_whole;  // tiles below are seen for their prefix, in part / whole
     int full;                  // tiles below hold 128 keys
@@ -233,16 +250,18 @@ struct TcItem {
     int from0, to0, whole_from0, whole_to0, from1, to1, whole_from1, whole_to1;
 };
 
+template <int KT>
 __device__ __forceinline__ void tile_range(const AttnDev &p, int first, int last, int kn, int &from, int &to, int &whole_from,
                                            int &whole_to)
 {
     const bool no_left = p.left == INT_MAX / 2, no_right = p.right == INT_MAX / 2;
-    from = no_left ? 0 : max(first - p.left, 0) / kTcKeys;
-    to = (max(no_right ? kn : min(kn, last + p.right + 1), 0) + kTcKeys - 1) / kTcKeys;
-    whole_from = no_left ? 0 : (max(last - p.left, 0) + kTcKeys - 1) / kTcKeys;
-    whole_to = no_right ? INT_MAX : max(first + p.right + 1, 0) / kTcKeys;
+    from = no_left ? 0 : max(first - p.left, 0) / KT;
+    to = (max(no_right ? kn : min(kn, last + p.right + 1), 0) + KT - 1) / KT;
+    whole_from = no_left ? 0 : (max(last - p.left, 0) + KT - 1) / KT;
+    whole_to = no_right ? INT_MAX : max(first + p.right + 1, 0) / KT;
 }
 
+template <int KT>
 __device__ __forceinline__ bool item_of(const AttnDev &p, int b, int h, int tile, TcItem &x)
 {
     x.b = b;
@@ -253,14 +272,17 @@ __device__ __forceinline__ bool item_of(const AttnDev &p, int b, int h, int tile
     if (x.row0 >= x.qn) return false;
     const int shift = p.align_end ? x.kn - x.qn : 0;
     const int pre = p.prefix ? min(max(__ldg(p.prefix + x.b), 0), x.kn) : 0;
+    x.doc_row = p.q_doc ? b % p.doc_rows : 0;
+    x.shift = shift;
+    x.pre = pre;
     x.both = x.row0 + 128 < x.qn;
     const int first = x.row0 + shift, last = min(x.row0 + 256, x.qn) - 1 + shift;
-    tile_range(p, first, x.both ? first + 127 : last, x.kn, x.from0, x.to0, x.whole_from0, x.whole_to0);
-    tile_range(p, first + 128, last, x.kn, x.from1, x.to1, x.whole_from1, x.whole_to1);
+    tile_range<KT>(p, first, x.both ? first + 127 : last, x.kn, x.from0, x.to0, x.whole_from0, x.whole_to0);
+    tile_range<KT>(p, first + 128, last, x.kn, x.from1, x.to1, x.whole_from1, x.whole_to1);
     if (!x.both) x.to1 = 0;
-    x.before = (pre + kTcKeys - 1) / kTcKeys;
-    x.before_whole = pre / kTcKeys;
-    x.full = x.kn / kTcKeys;
+    x.before = (pre + KT - 1) / KT;
+    x.before_whole = pre / KT;
+    x.full = x.kn / KT;
     x.t0 = x.before ? 0 : x.both ? min(x.from0, x.from1) : x.from0;
     x.t1 = max(max(x.before, x.to0), x.to1);
     return true;
@@ -285,13 +307,13 @@ struct TcWalk {
             b -= h * P.a.batch;
         }
     }
-    __device__ __forceinline__ bool next(const TcDev &P, TcItem &x)
+    template <int KT> __device__ __forceinline__ bool next(const TcDev &P, TcItem &x)
     {
         const AttnDev &p = P.a;
         while (at < end) {
             bool found;
             if (P.head_major) {
-                found = item_of(p, b, h, tile, x);
+                found = item_of<KT>(p, b, h, tile, x);
                 at++;
                 if (++tile == P.tiles) {
                     tile = 0;
@@ -306,7 +328,7 @@ struct TcWalk {
                 at += gridDim.x;
                 if (item >= end) continue;
                 const uint32_t row = item / p.hq, last = row / p.batch;
-                found = item_of(p, row - last * p.batch, item - row * p.hq, P.tiles - 1 - (int)last, x);
+                found = item_of<KT>(p, row - last * p.batch, item - row * p.hq, P.tiles - 1 - (int)last, x);
             }
             if (found) return true;
         }
@@ -322,11 +344,12 @@ __device__ __forceinline__ bool tc_active(const TcItem &x, const uint32_t *bits,
 }
 
 template <typename T, int DP, int FORM>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
     k_attn_tc(const __grid_constant__ TcDev P, const __grid_constant__ CUtensorMap mq,
               const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv)
 {
     using C = TcCfg<DP>;
+    constexpr int KT = C::KT;
     const AttnDev &p = P.a;
     extern __shared__ char sm_raw[];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -335,20 +358,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t bars = s0 + C::BARS;
     const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * C::ST,
                    v_full = k_empty + 8 * C::ST, v_empty = v_full + 8 * C::ST, s_full = v_empty + 8 * C::ST,
-                   s_empty = s_full + 16, p_full = s_empty + 16, p_empty = p_full + 16, o_full = p_empty + 16,
-                   bits_full = o_full + 16, bits_empty = bits_full + 16, go = bits_empty + 16,
-                   p_half = go + 64;
+                   p_full = s_full + 16, o_full = p_full + 16,
+                   item_full = o_full + 16, item_empty = item_full + 16, go = item_empty + 16,
+                   p_half = go + 64, meet = p_half + 16;
     uint32_t *const tmem_at = (uint32_t *)(sm + C::BARS + C::NBAR * 8);
+    TcItem *const items = (TcItem *)(sm + C::ITEMS);
+    static_assert(sizeof(TcItem) <= 128, "");
     uint32_t *const bit_sets = (uint32_t *)(sm + C::MORE);
 
     if (warp == 9) {
-        tmem_alloc(smem_u32(tmem_at), 512);
+        tmem_alloc(smem_u32(tmem_at), C::COLUMNS);
     } else if (tid == 256) {
         tma_prefetch_desc(&mq);
         tma_prefetch_desc(&mk);
         tma_prefetch_desc(&mv);
-        for (uint32_t x = bars; x < p_half + 16; x += 8)
-            mbar_init(x, x >= p_half ? 4 : x >= go ? 1 : x >= bits_empty ? 11 : x >= s_empty && x < p_empty ? 4 : x >= k_empty && x < v_full || x >= v_empty && x < s_full ? 2 : 1);
+        for (uint32_t x = bars; x < meet + 16; x += 8)
+            mbar_init(x, x >= p_half ? 4 : x >= go ? 1 : x >= item_empty ? 11 : x >= item_full ? 1 : x >= p_full && x < o_full ? 4 : x >= k_empty && x < v_full || x >= v_empty && x < s_full ? 2 : 1);
         fence_mbar_init();
     }
     tc_fence_before();
@@ -356,32 +381,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
     const bool documents = p.q_doc != nullptr;
-    TcWalk walk;
-    TcItem x;
-    walk.start(P);
-    int turn = 0;  // items so far (their bit sets alternate)
+    int turn = 0;  // items so far (their places in shared memory alternate)
     bool ok = true;
+    // The next item, from warp 11; done() gives its place back.
+    TcItem x;
+    auto next = [&]() {
+        if (!(ok = tc_wait(item_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) return false;
+        x = items[turn & 1];
+        return x.b >= 0;
+    };
+    auto done = [&]() { mbar_arrive(item_empty + 8 * (turn & 1)); };
     auto bits_of = [&](int n) { return documents ? bit_sets + (n & 1) * P.words * 4 : nullptr; };
 
     // 384 threads of 168 registers: the softmax warps take 216 (a row of 128 scores and more), 72 stay
     // for the copies, the products and the documents.
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (C::BLOCKS == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_REST));
         if (warp == 8) {
             // ---- copies ----
             if (elect_one()) {
                 int n = 0, nq[2] = {0, 0};
                 bool v_here = true;  // whether the last keys' values were asked for as well
-                for (; ok && walk.next(P, x); turn++) {
+                for (; next(); turn++) {
                     const uint32_t *bits = bits_of(turn);
-                    if (bits && !(ok = tc_wait(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
                     const int g = x.h / p.group;
                     bool q_here[2] = {false, false};
                     auto queries = [&](int q) {
                         if (q_here[q] || !(ok = tc_wait(q_empty + 8 * q, (nq[q] & 1) ^ 1, P.err, 200))) return;
-                        mbar_arrive_expect_tx(q_full + 8 * q, C::TILE);
+                        mbar_arrive_expect_tx(q_full + 8 * q, C::QTILE);
                         for (int y = 0; y < DP / 64; y++)
-                            tma_load_4d(s0 + C::Q + q * C::TILE + y * 16384, &mq, q_full + 8 * q, 64 * y, x.row0 + 128 * q, x.h,
+                            tma_load_4d(s0 + C::Q + q * C::QTILE + y * 16384, &mq, q_full + 8 * q, 64 * y, x.row0 + 128 * q, x.h,
                                         x.b);
                         q_here[q] = true;
                         nq[q]++;
@@ -395,17 +424,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (!ok || !(ok = tc_wait(k_empty + 8 * st, parity, P.err, 201))) break;
                         mbar_arrive_expect_tx(k_full + 8 * st, C::TILE);
                         for (int y = 0; y < DP / 64; y++)
-                            tma_load_4d(s0 + C::K + st * C::TILE + y * 16384, &mk, k_full + 8 * st, 64 * y, t * kTcKeys, g, x.b);
+                            tma_load_4d(s0 + C::K + st * C::TILE + y * C::HALF, &mk, k_full + 8 * st, 64 * y, t * KT, g, x.b);
                         n++;
                         v_here = false;
                         if (act[1]) queries(1);
                         if (!ok || !(ok = tc_wait(v_empty + 8 * st, parity, P.err, 202))) break;
                         mbar_arrive_expect_tx(v_full + 8 * st, C::TILE);
                         for (int y = 0; y < DP / 64; y++)
-                            tma_load_4d(s0 + C::V + st * C::TILE + y * 16384, &mv, v_full + 8 * st, 64 * y, t * kTcKeys, g, x.b);
+                            tma_load_4d(s0 + C::V + st * C::TILE + y * C::HALF, &mv, v_full + 8 * st, 64 * y, t * KT, g, x.b);
                         v_here = true;
                     }
-                    if (bits) mbar_arrive(bits_empty + 8 * (turn & 1));
+                    if (!ok) break;
+                    done();
                 }
                 // every copy has landed before the block ends, also where a wait gave up
 #pragma unroll
@@ -421,53 +451,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int q = warp - 9;
             // N of P V: the components, in sixteens; k of Q K^T likewise
             const int dn = (p.d + 15) / 16 * 16;
-            const uint32_t id_s = idesc_of<T>(128, false), id_o = idesc_of<T>(dn, true);
-            const uint32_t s_at = tmem + 128 * q, p_at = tmem + C::P_AT + C::P_Q * q, o_at = tmem + C::O_AT + C::O_Q * q;
-            const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::TILE, 16);
-            uint32_t phase = 0;  // of p_full (bit 0), q_full (1), s_empty (2) and p_half (3)
+            const uint32_t id_s = idesc_of<T>(KT, false), id_o = idesc_of<T>(dn, true);
+            const uint32_t s_at = tmem + KT * q, o_at = tmem + 2 * KT + DP * q;
+            const uint64_t qd = swizzled_desc(s0 + C::Q + q * C::QTILE, 16);
+            uint32_t phase = 0;  // of p_full (bit 0), q_full (1) and p_half (2)
             auto wait = [&](uint32_t bar, int bit, int code) {
                 const bool done = tc_wait_warp(bar + 8 * q, phase >> bit & 1, P.err, code);
                 phase ^= 1u << bit;
                 return done;
             };
             int n = 0;            // key tiles so far, of both query tiles
-            bool made = false;    // scores were computed before: their columns are to be free again
-            for (; ok && walk.next(P, x); turn++) {
+            for (; __all_sync(0xffffffffu, next()); turn++) {
                 const uint32_t *bits = bits_of(turn);
-                if (bits && !(ok = tc_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) break;
                 bool q_here = false, acc = false;
                 int n_pend = -1, t_pend = 0;  // the key tile whose scores the softmax warps have
                 // O += P V of that key tile
                 auto values = [&]() {
                     const int st = n_pend % C::ST;
                     if (!tc_wait_warp(v_full + 8 * st, (n_pend / C::ST) & 1, P.err, 206)) return false;
-                    const int live = x.kn - t_pend * kTcKeys;
-                    if (live < kTcKeys && x.kn < p.lk) {
+                    const int live = x.kn - t_pend * KT;
+                    if (live < KT && x.kn < p.lk) {
                         // values behind the last key may be anything: zeros (from both warps), as 0 * NaN is NaN
-                        for (int i = lane; i < (kTcKeys - live) * (DP / 8); i += 32) {
+                        for (int i = lane; i < (KT - live) * (DP / 8); i += 32) {
                             const int r = live + i / (DP / 8), c = i % (DP / 8);
-                            *reinterpret_cast<uint4 *>(sm + C::V + st * C::TILE + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) =
+                            *reinterpret_cast<uint4 *>(sm + C::V + st * C::TILE + (c >> 3) * C::HALF + r * 128 + (c & 7) * 16) =
                                 make_uint4(0, 0, 0, 0);
                         }
                         fence_proxy_async();
                         __syncwarp();
                     }
-                    const uint64_t vd = swizzled_desc(s0 + C::V + st * C::TILE, 16384);
-                    if (!wait(p_half, 3, 218)) return false;
+                    const uint64_t vd = swizzled_desc(s0 + C::V + st * C::TILE, C::HALF);
+                    if (!wait(p_half, 2, 218)) return false;
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < kTcKeys / 32; kk++)
-                            mma_f16_ts(o_at, p_at + 8 * kk, vd + (kk * 2048 >> 4), id_o, acc || kk > 0);
+                        for (int kk = 0; kk < KT / 32; kk++)
+                            mma_f16_ts(o_at, s_at + 8 * kk, vd + (kk * 2048 >> 4), id_o, acc || kk > 0);
                     }
                     __syncwarp();
                     if (!wait(p_full, 0, 207)) return false;
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = kTcKeys / 32; kk < kTcKeys / 16; kk++)
-                            mma_f16_ts(o_at, p_at + 8 * kk, vd + (kk * 2048 >> 4), id_o, 1u);
-                        if (C::APART) mma_commit(p_empty + 8 * q);
+                        for (int kk = KT / 32; kk < KT / 16; kk++)
+                            mma_f16_ts(o_at, s_at + 8 * kk, vd + (kk * 2048 >> 4), id_o, 1u);
                         mma_commit(v_empty + 8 * st);
                     }
                     __syncwarp();
@@ -480,29 +507,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (!mine && !tc_active(x, bits, 1 - q, t)) continue;
                     const int st = n % C::ST;
                     if (mine) {
-                        // the scores' columns: free once the product with the values that reads them is issued, or (APART)
-                        // once they are in registers
-                        if (!C::APART && n_pend >= 0 && !(ok = values())) break;
+                        // (the scores' columns are free once the product that reads them as probabilities is issued)
+                        if (n_pend >= 0 && !(ok = values())) break;
                         if (!q_here && !(ok = wait(q_full, 1, 209))) break;
                         q_here = true;
                         if (!(ok = tc_wait_warp(k_full + 8 * st, (n / C::ST) & 1, P.err, 208))) break;
-                        if (C::APART && made) {
-                            if (!(ok = wait(s_empty, 2, 215))) break;
-                            tc_fence_after();
-                        }
-                        made = true;
                         if (elect_one()) {
                             const uint64_t kd = swizzled_desc(s0 + C::K + st * C::TILE, 16);
 #pragma unroll
                             for (int kk = 0; kk < DP / 16; kk++) {
-                                const uint32_t at = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-                                if (kk * 16 < p.d) mma_f16(s_at, qd + at, kd + at, id_s, kk > 0, 0);
+                                const uint32_t qa = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4, ka = ((kk >> 2) * C::HALF + (kk & 3) * 32) >> 4;
+                                if (kk * 16 < p.d) mma_f16(s_at, qd + qa, kd + ka, id_s, kk > 0, 0);
                             }
                             mma_commit(s_full + 8 * q);
                             mma_commit(k_empty + 8 * st);
                         }
                         __syncwarp();
-                        if (C::APART && n_pend >= 0 && !(ok = values())) break;
                         n_pend = n;
                         t_pend = t;
                     } else {
@@ -523,8 +543,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (ok && q_here && elect_one()) mma_commit(q_empty + 8 * q);
                 if (ok && n_pend >= 0) ok = values();
                 if (ok && acc && elect_one()) mma_commit(o_full + 8 * q);
-                if (bits && lane == 0) mbar_arrive(bits_empty + 8 * (turn & 1));
+                if (!ok) break;
                 __syncwarp();
+                if (lane == 0) done();
             }
             // no product is in flight when the block ends (the softmax warps do not wait where a wait gave up)
             if (!ok) {
@@ -532,74 +553,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 for (int i = 0; i < 2; i++) tc_wait_warp(o_full + 8 * q, i, P.err, 212);
             }
-        } else if (documents) {
-            // ---- documents: which key tiles hold one of a query tile's, and which nothing but its only one ----
-            for (; ok && walk.next(P, x); turn++) {
-                if (!(ok = tc_wait_warp(bits_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214))) break;
-                uint32_t *bits = bit_sets + (turn & 1) * P.words * 4;
-                const int *qd = p.q_doc + (int64_t)(x.b % p.doc_rows) * p.lq, *kd = p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk;
-                int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
+        } else {
+            // ---- items, and documents: which key tiles hold one of a query tile's, and which nothing but its only one ----
+            TcWalk walk;
+            walk.start(P);
+            for (;; turn++) {
+                const bool more = walk.next<KT>(P, x);
+                if (!more) x.b = -1;
+                if (!tc_wait_warp(item_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214)) break;
+                if (lane == 0) items[turn & 1] = x;
+                if (more && documents) {
+                    uint32_t *bits = bit_sets + (turn & 1) * P.words * 4;
+                    const int *qd = p.q_doc + (int64_t)(x.b % p.doc_rows) * p.lq, *kd = p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk;
+                    int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
 #pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const int i = x.row0 + 32 * y + lane;
-                    if (i < x.qn) {
-                        const int id = __ldg(qd + i);
-                        lo[y >> 2] = min(lo[y >> 2], id);
-                        hi[y >> 2] = max(hi[y >> 2], id);
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    lo[q] = __reduce_min_sync(0xffffffffu, lo[q]);
-                    hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
-                }
-                const int word0 = x.t0 / 32;
-                for (int w = word0; w * 32 < x.t1; w++) {
-                    int klo = INT_MAX, khi = INT_MIN;
-                    for (int y = max(x.t0 - w * 32, 0); y < min(x.t1 - w * 32, 32); y += 4) {
-                        // four tiles' loads in flight; lane l keeps tile l's range
-                        int a[4], z[4];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            a[u] = INT_MAX, z[u] = INT_MIN;
-#pragma unroll
-                            for (int v = 0; v < kTcKeys / 32; v++) {
-                                const int j = (w * 32 + y + u) * kTcKeys + v * 32 + lane;
-                                if (j < x.kn) {
-                                    const int id = __ldg(kd + j);
-                                    a[u] = min(a[u], id);
-                                    z[u] = max(z[u], id);
-                                }
-                            }
-                        }
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            const int aa = __reduce_min_sync(0xffffffffu, a[u]), zz = __reduce_max_sync(0xffffffffu, z[u]);
-                            if (lane == y + u) klo = aa, khi = zz;
+                    for (int y = 0; y < 8; y++) {
+                        const int i = x.row0 + 32 * y + lane;
+                        if (i < x.qn) {
+                            const int id = __ldg(qd + i);
+                            lo[y >> 2] = min(lo[y >> 2], id);
+                            hi[y >> 2] = max(hi[y >> 2], id);
                         }
                     }
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
-                        const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo[q], 0) <= khi && klo <= hi[q]);
-                        const uint32_t only =
-                            __ballot_sync(0xffffffffu, lo[q] >= 0 && lo[q] == hi[q] && klo == lo[q] && khi == lo[q]);
-                        if (lane == 0) {
-                            bits[4 * (w - word0) + q] = seen;
-                            bits[4 * (w - word0) + 2 + q] = only;
+                        lo[q] = __reduce_min_sync(0xffffffffu, lo[q]);
+                        hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
+                    }
+                    const int word0 = x.t0 / 32;
+                    for (int w = word0; w * 32 < x.t1; w++) {
+                        int klo = INT_MAX, khi = INT_MIN;
+    constexpr int U = 16 * 32 / KT;
+                                        for (int y = max(x.t0 - w * 32, 0); y < min(x.t1 - w * 32, 32); y += U) {
+                            // U tiles' loads in flight; lane l keeps tile l's range
+                            int a[U], z[U];
+#pragma unroll
+                            for (int u = 0; u < U; u++) {
+                                a[u] = INT_MAX, z[u] = INT_MIN;
+#pragma unroll
+                                for (int v = 0; v < KT / 32; v++) {
+                                    const int j = (w * 32 + y + u) * KT + v * 32 + lane;
+                                    if (j < x.kn) {
+                                        const int id = __ldg(kd + j);
+                                        a[u] = min(a[u], id);
+                                        z[u] = max(z[u], id);
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int u = 0; u < U; u++) {
+                                const int aa = __reduce_min_sync(0xffffffffu, a[u]), zz = __reduce_max_sync(0xffffffffu, z[u]);
+                                if (lane == y + u) klo = aa, khi = zz;
+                            }
+                        }
+#pragma unroll
+                        for (int q = 0; q < 2; q++) {
+                            const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo[q], 0) <= khi && klo <= hi[q]);
+                            const uint32_t only =
+                                __ballot_sync(0xffffffffu, lo[q] >= 0 && lo[q] == hi[q] && klo == lo[q] && khi == lo[q]);
+                            if (lane == 0) {
+                                bits[4 * (w - word0) + q] = seen;
+                                bits[4 * (w - word0) + 2 + q] = only;
+                            }
                         }
                     }
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bits_full + 8 * (turn & 1));
+                if (lane == 0) mbar_arrive(item_full + 8 * (turn & 1));
+                if (!more) break;
             }
         }
     } else {
         // ---- softmax ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if (C::BLOCKS == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
         const int q = warp >> 2, r_in = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + 128 * q, p_at = tmem + lanes + C::P_AT + C::P_Q * q,
-                       o_at = tmem + lanes + C::O_AT + C::O_Q * q;
+        const uint32_t s_at = tmem + lanes + KT * q, o_at = tmem + lanes + 2 * KT + DP * q;
         const bool grid = FORM == kFormGrid || (FORM == kFormAny && P.bias_form == kBiasGridDirect);
         const bool capped = FORM == kFormCap || (FORM == kFormAny && p.cap_out > 0.f);
         const bool scaled = FORM != kFormPlain && (FORM != kFormAny || P.scaled);
@@ -612,7 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (grid) {
             // where a key's (grids a multiple of 4 wide: four keys') entry of the table is, from its query's;
             // behind the last key: the first's, which is masked
-            for (int j = tid; j < (p.lk + 127) / 128 * 128; j += 256) {
+            for (int j = tid; j < (p.lk + KT - 1) / KT * KT; j += 256) {
                 const int jj = j < p.lk ? j : 0, y = jj / p.grid_w, at = y * P.table_st + jj - y * p.grid_w;
                 if (!quads)
                     places[j] = at;
@@ -621,9 +650,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             named_bar_sync(3, 256);
         }
-        constexpr int CH = 32;
-        uint32_t s_phase = 0, o_phase = 0, p_phase = 0;
-        bool p_made = false;  // probabilities were handed on before
+        // Two blocks an SM: 80 registers hold 32 scores of a row at a time, read twice. One: the whole row.
+        constexpr bool TWICE = C::BLOCKS == 2, TURNS = C::BLOCKS == 1;
+        constexpr int CH = 32, W = TWICE ? 32 : KT;
+        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t meets = 0;
+        auto together = [&]() {  // the four warps of this query tile (bounded, unlike bar.sync)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(meet + 8 * q);
+            return tc_wait_warp(meet + 8 * q, meets++ & 1, P.err, 219);
+        };
         // Warps w and w + 4 share a scheduler and its exponential unit (4 a cycle): they take turns, so that
         // one's exponentials run beside the other's products, loads and maxima and not beside its exponentials.
         uint32_t turns = q ? 0 : 1;
@@ -636,25 +672,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(go + 8 * (warp ^ 4));
         };
-        for (; walk.next(P, x); turn++) {
+        for (; __all_sync(0xffffffffu, next()); turn++) {
             if (grid && table_h != x.h) {
-                // (a warp whose wait gave up still comes to these barriers)
-                named_bar_sync(1 + q, 128);
+                if (!(ok = together())) break;  // nobody reads the last head's any more
                 const float *src = p.bias_data + (int64_t)x.h * (2 * p.reach_y + 1) * (2 * p.reach_x + 1);
                 for (int e = tid & 127; e < table_n; e += 128) {
                     const int y = e / P.table_st, c = e - y * P.table_st;
                     if (c <= 2 * p.reach_x) table[e] = __ldg(src + y * (2 * p.reach_x + 1) + c) * kLog2e;
                 }
-                named_bar_sync(1 + q, 128);
+                if (!(ok = together())) break;
                 table_h = x.h;
             }
-            if (!ok) continue;
             const uint32_t *bits = bits_of(turn);
-            if (bits && !(ok = tc_wait_warp(bits_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) continue;
             const int i = x.row0 + 128 * q + r_in;
             const bool there = i < x.qn;
-            const Query r = query_of(p, x.b, x.h, min(i, x.qn - 1), x.qn, x.kn);
-            const int *const docs = documents ? p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk : nullptr;
+            const Query r = query_at(p, x.doc_row, x.h, min(i, x.qn - 1), x.shift, x.pre);
+            const int *const docs = documents ? p.k_doc + (int64_t)x.doc_row * p.lk : nullptr;
             const float *const mine = table + (p.reach_y - r.y) * P.table_st + p.reach_x - r.x;
             const int from = q ? x.from1 : x.from0, to = q ? x.to1 : x.to0, before = q && !x.both ? 0 : x.before;
             const int whole_from = q ? x.whole_from1 : x.whole_from0, whole_to = q ? x.whole_to1 : x.whole_to0;
@@ -670,21 +703,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 if (!seen_here) {
                     // the other query tile's alone: pass its turn on
-                    if (x.both && tc_active(x, bits, 1 - q, t)) {
+                    if (TURNS && x.both && tc_active(x, bits, 1 - q, t)) {
                         if (!(ok = my_turn())) break;
                         pass_turn();
                     }
                     continue;
                 }
-                const int j0 = t * kTcKeys;
+                const int j0 = t * KT;
                 if (!(ok = tc_wait_warp(s_full + 8 * q, s_phase, P.err, 210))) break;
                 s_phase ^= 1;
                 tc_fence_after();
                 // Scores that are more than a scaled product are made in a first pass, CH columns at a time (a short
                 // loop: unrolled over the row its instructions are fetched anew every time), and put back.
-                if (scaled || !all) {
+                const bool back = scaled || !all;
+                float now = -INFINITY;
+                if (TWICE || back) {
 #pragma unroll 1
-                for (int c0 = 0; c0 < kTcKeys; c0 += CH) {
+                for (int c0 = 0; c0 < KT; c0 += CH) {
                     float s[CH];
 #pragma unroll
                     for (int c = 0; c < CH; c += 32) tmem_ld32(s_at + c0 + c, s + c);
@@ -762,42 +797,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int c = 0; c < 32; c++) s[w + c] = seen >> c & 1 ? s[w + c] : -INFINITY;
                         }
                     }
+                    if (TWICE) now = fmaxf(now, row_max<CH>(s));
+                    if (back) {
 #pragma unroll
-                    for (int c = 0; c < CH; c += 16) {
-                        uint32_t w[16];
+                        for (int c = 0; c < CH; c += 16) {
+                            uint32_t w[16];
 #pragma unroll
-                        for (int y = 0; y < 16; y++) w[y] = __float_as_uint(s[c + y]);
-                        tmem_st16(s_at + c0 + c, w);
+                            for (int y = 0; y < 16; y++) w[y] = __float_as_uint(s[c + y]);
+                            tmem_st16(s_at + c0 + c, w);
+                        }
                     }
                 }
-                tmem_wait_st();
+                if (back) tmem_wait_st();
                 }
-                float s[kTcKeys];
+                float s[W];
+                if (!TWICE) {
 #pragma unroll
-                for (int c = 0; c < kTcKeys; c += 32) tmem_ld32(s_at + c, s + c);
-                tmem_wait_ld();
-                if (C::APART) {
-                    // the scores are in registers: their columns are free
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(s_empty + 8 * q);
+                    for (int c = 0; c < W; c += 32) tmem_ld32(s_at + c, s + c);
+                    tmem_wait_ld();
+                    now = row_max<W>(s);
                 }
-                float top[4];
-#pragma unroll
-                for (int y = 0; y < 4; y++) {
-                    top[y] = s[y];
-#pragma unroll
-                    for (int c = 4 + y; c < kTcKeys - 4; c += 8) top[y] = max3(top[y], s[c], s[c + 4]);
-                    top[y] = fmaxf(top[y], s[kTcKeys - 4 + y]);
-                }
-                const float now = max3(fmaxf(top[0], top[1]), top[2], top[3]);
-                if (C::APART && p_made) {
-                    // the product before is done with the probabilities and the outputs
-                    if (!(ok = tc_wait_warp(p_empty + 8 * q, p_phase, P.err, 216))) break;
-                    p_phase ^= 1;
-                    tc_fence_after();
-                }
-                p_made = true;
                 // (m is -inf until a row has seen a key)
                 if (__any_sync(0xffffffffu, now * sc > m * sc + 8.f || (m == -INFINITY && now > m))) {
                     const float to = fmaxf(m, now), alpha = exp2_fast((m - (to == -INFINITY ? 0.f : to)) * sc);
@@ -819,35 +838,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 any = true;
                 const float base = m == -INFINITY ? 0.f : m * sc;
                 const F2 sc2 = f2(sc, sc), base2 = f2(-base, -base);
-#pragma unroll
-                for (int c = 0; c < kTcKeys; c += 2) f2_out(f2_fma(f2(s[c], s[c + 1]), sc2, base2), s[c], s[c + 1]);
-                if (x.both && !(ok = my_turn())) break;
                 F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-                for (int c = 0; c < kTcKeys; c += 32) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int y = 0; y < 16; y++) {
-                        F2 e;
-                        if (y % 4 == 3)  // a quarter of them on the FMA pipe
-                            e = f2_exp2(s[c + 2 * y], s[c + 2 * y + 1]);
-                        else
-                            e = f2(exp2_fast(s[c + 2 * y]), exp2_fast(s[c + 2 * y + 1]));
-                        sum[y & 1] = f2_add(sum[y & 1], e);
-                        float a, z;
-                        f2_out(e, a, z);
-                        w[y] = MmaOp<T>::pack(a, z);
+#pragma unroll 1
+                for (int c0 = 0; c0 < KT; c0 += W) {
+                    if (TWICE) {
+                        tmem_ld32(s_at + c0, s);
+                        tmem_wait_ld();
                     }
-                    tmem_st16(p_at + c / 2, w);
-                    if (c == kTcKeys / 2 - 32) {
-                        // the product with the first half of the values can start
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(p_half + 8 * q);
+#pragma unroll
+                    for (int c = 0; c < W; c += 2) f2_out(f2_fma(f2(s[c], s[c + 1]), sc2, base2), s[c], s[c + 1]);
+                    if (TURNS && x.both && !(ok = my_turn())) break;
+#pragma unroll
+                    for (int c = 0; c < W; c += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int y = 0; y < 16; y++) {
+                            F2 e;
+                            if (!TWICE && y % 4 == 3)  // a quarter of them on the FMA pipe
+                                e = f2_exp2(s[c + 2 * y], s[c + 2 * y + 1]);
+                            else
+                                e = f2(exp2_fast(s[c + 2 * y]), exp2_fast(s[c + 2 * y + 1]));
+                            sum[y & 1] = f2_add(sum[y & 1], e);
+                            float a, z;
+                            f2_out(e, a, z);
+                            w[y] = MmaOp<T>::pack(a, z);
+                        }
+                        tmem_st16(s_at + (c0 + c) / 2, w);
+                        if (c0 + c == KT / 2 - 32) {
+                            // the product with the first half of the values can start
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(p_half + 8 * q);
+                        }
                     }
+                    if (TURNS && x.both) pass_turn();
                 }
-                if (x.both) pass_turn();
+                if (!ok) break;
                 float la, lb;
                 f2_out(f2_add(sum[0], sum[1]), la, lb);
                 l += la + lb;
@@ -856,19 +883,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + 8 * q);
             }
-            if (bits) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bits_empty + 8 * (turn & 1));
-            }
-            if (!ok) continue;
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) done();
 
             // ---- out: a thread a row ----
             if (any) {
-                if (!(ok = tc_wait_warp(o_full + 8 * q, o_phase, P.err, 211))) continue;
+                if (!(ok = tc_wait_warp(o_full + 8 * q, o_phase, P.err, 211))) break;
                 o_phase ^= 1;
                 tc_fence_after();
             }
             if (q && !x.both) continue;
+            // (what a query without keys has accumulated is 0 * v: not finite only where the row is taken again)
             const float f = l == 0.f ? 0.f : 1.f / l;
             T *const dst = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)i * p.ot;
             bool odd = false;
@@ -877,16 +903,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (any) {
                     tmem_ld32(o_at + c, o);
                     tmem_wait_ld();
-                }
+                } else {
 #pragma unroll
-                for (int y = 0; y < 32; y++) {
-                    if (!any) o[y] = 0.f;
-                    if (c + y < p.d) odd |= !(fabsf(o[y]) < INFINITY);
-                    o[y] = l == 0.f ? 0.f : o[y] * f;
+                    for (int y = 0; y < 32; y++) o[y] = 0.f;
+                }
+                if (p.masked) {
+                    // a sum of zeros, unless something is not finite
+                    float z = 0.f;
+#pragma unroll
+                    for (int y = 0; y < 32; y++)
+                        if (c + (y & ~15) < p.d) z = fmaf(o[y], 0.f, z);
+                    odd |= z != 0.f;
                 }
                 uint32_t w[16];
+                const F2 ff = f2(f, f);
 #pragma unroll
-                for (int y = 0; y < 16; y++) w[y] = MmaOp<T>::pack(o[2 * y], o[2 * y + 1]);
+                for (int y = 0; y < 16; y++) {
+                    f2_out(f2_mul(f2(o[2 * y], o[2 * y + 1]), ff), o[2 * y], o[2 * y + 1]);
+                    w[y] = MmaOp<T>::pack(o[2 * y], o[2 * y + 1]);
+                }
                 if (!there) continue;
                 // (d is a multiple of 8, of 16 where 32-byte stores are allowed)
                 if (P.wo == 32) {
@@ -915,7 +950,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (; again; again &= again - 1) {
                 const int row = x.row0 + 128 * q + (warp & 3) * 32 + __ffs(again) - 1;
                 float rm, rl, ro[8];
-                attend_row<T>(p, x.b, x.h, row, x.qn, x.kn, x.t0 * kTcKeys, min(x.t1 * kTcKeys, x.kn),
+                attend_row<T>(p, x.b, x.h, row, x.qn, x.kn, x.t0 * KT, min(x.t1 * KT, x.kn),
                               (float *)(sm + C::SCRATCH) + warp * 256, rm, rl, ro);
                 const float rf = rl == 0.f ? 0.f : 1.f / rl;
                 T *const to = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)row * p.ot;
@@ -929,7 +964,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     if (warp == 9) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, C::COLUMNS);
     }
 }
 

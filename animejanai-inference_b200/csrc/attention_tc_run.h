@@ -41,7 +41,7 @@ cudaError_t run_tc(TcDev &p, const ajib_attn *op, const CUtensorMap (&m)[3], cud
     if (e != cudaSuccess) return e;
     p.words = TcCfg<DP>::bit_words(op);
     p.table_st = TcCfg<DP>::table_stride(op);
-    const unsigned blocks = (unsigned)std::min<int64_t>(p.items, sm_count());
+    const unsigned blocks = (unsigned)std::min<int64_t>(p.items, sm_count() * TcCfg<DP>::BLOCKS);
     dev::k_attn_tc<T, DP, FORM><<<blocks, kTcThreads, (int)TcCfg<DP>::smem(op), s>>>(p, m[0], m[1], m[2]);
     return cudaGetLastError();
 }
