@@ -241,7 +241,7 @@ __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? ~0u : n
 struct __align__(16) TcItem {
     int b, h, row0, qn, kn;    // b < 0: no more items
     int shift, pre;            // query i stands at i + shift; keys below pre are seen by all
-    int doc_row;
+    int doc_row, word0;        // of documents: their row, and the first word of the bit sets
     int both;                  // there are queries in the second tile
     int t0, t1;                // key tiles that any query sees
     int before, before_whole;  // tiles below are seen for their prefix, in part / whole
@@ -285,6 +285,7 @@ __device__ __forceinline__ bool item_of(const AttnDev &p, int b, int h, int tile
     x.full = x.kn / KT;
     x.t0 = x.before ? 0 : x.both ? min(x.from0, x.from1) : x.from0;
     x.t1 = max(max(x.before, x.to0), x.to1);
+    x.word0 = x.t0 / 32;
     return true;
 }
 
@@ -340,7 +341,70 @@ struct TcWalk {
 __device__ __forceinline__ bool tc_active(const TcItem &x, const uint32_t *bits, int q, int t)
 {
     const bool reach = t < x.before ? !q || x.both : q ? t >= x.from1 && t < x.to1 : t >= x.from0 && t < x.to0;
-    return reach && !(bits && !(bits[4 * (t / 32 - x.t0 / 32) + q] >> (t & 31) & 1));
+    return reach && !(bits && !(bits[4 * (t / 32 - x.word0) + q] >> (t & 31) & 1));
+}
+
+// The bit sets of an item's documents, and its key tiles narrowed to those between the first and the
+// last that holds one. One warp, a lane a key tile.
+template <int KT> __device__ __forceinline__ void document_tiles(const AttnDev &p, TcItem &x, uint32_t *bits)
+{
+    const int lane = threadIdx.x & 31;
+    const int *qd = p.q_doc + (int64_t)x.doc_row * p.lq, *kd = p.k_doc + (int64_t)x.doc_row * p.lk;
+    int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
+#pragma unroll
+    for (int y = 0; y < 8; y++) {
+        const int i = x.row0 + 32 * y + lane;
+        if (i < x.qn) {
+            const int id = __ldg(qd + i);
+            lo[y >> 2] = min(lo[y >> 2], id);
+            hi[y >> 2] = max(hi[y >> 2], id);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        lo[q] = __reduce_min_sync(0xffffffffu, lo[q]);
+        hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
+    }
+    const bool wide = ((uintptr_t)kd & 15) == 0;
+    int t_first = x.t1, t_last = x.t0 - 1;
+    for (int w = x.word0; w * 32 < x.t1; w++) {
+        const int t = w * 32 + lane, j = t * KT, n = min(x.kn - j, KT);
+        int klo = INT_MAX, khi = INT_MIN;
+        if (t >= x.t0 && t < x.t1) {
+            if (wide && n == KT) {
+#pragma unroll 8
+                for (int v = 0; v < KT; v += 4) {
+                    const int4 id = __ldg(reinterpret_cast<const int4 *>(kd + j + v));
+                    klo = min(min(klo, min(id.x, id.y)), min(id.z, id.w));
+                    khi = max(max(khi, max(id.x, id.y)), max(id.z, id.w));
+                }
+            } else {
+#pragma unroll 8
+                for (int v = 0; v < n; v++) {
+                    const int id = __ldg(kd + j + v);
+                    klo = min(klo, id);
+                    khi = max(khi, id);
+                }
+            }
+        }
+        uint32_t either = 0;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo[q], 0) <= khi && klo <= hi[q]);
+            const uint32_t only = __ballot_sync(0xffffffffu, lo[q] >= 0 && lo[q] == hi[q] && klo == lo[q] && khi == lo[q]);
+            if (lane == 0) {
+                bits[4 * (w - x.word0) + q] = seen;
+                bits[4 * (w - x.word0) + 2 + q] = only;
+            }
+            either |= seen;
+        }
+        if (either) {
+            t_first = min(t_first, w * 32 + __ffs(either) - 1);
+            t_last = max(t_last, w * 32 + 31 - __clz(either));
+        }
+    }
+    x.t0 = min(t_first, x.t1);
+    x.t1 = t_last + 1;
 }
 
 template <typename T, int DP, int FORM>
@@ -561,63 +625,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                 const bool more = walk.next<KT>(P, x);
                 if (!more) x.b = -1;
                 if (!tc_wait_warp(item_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214)) break;
+                if (more && documents) document_tiles<KT>(p, x, bit_sets + (turn & 1) * P.words * 4);
                 if (lane == 0) items[turn & 1] = x;
-                if (more && documents) {
-                    uint32_t *bits = bit_sets + (turn & 1) * P.words * 4;
-                    const int *qd = p.q_doc + (int64_t)(x.b % p.doc_rows) * p.lq, *kd = p.k_doc + (int64_t)(x.b % p.doc_rows) * p.lk;
-                    int lo[2] = {INT_MAX, INT_MAX}, hi[2] = {INT_MIN, INT_MIN};
-#pragma unroll
-                    for (int y = 0; y < 8; y++) {
-                        const int i = x.row0 + 32 * y + lane;
-                        if (i < x.qn) {
-                            const int id = __ldg(qd + i);
-                            lo[y >> 2] = min(lo[y >> 2], id);
-                            hi[y >> 2] = max(hi[y >> 2], id);
-                        }
-                    }
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        lo[q] = __reduce_min_sync(0xffffffffu, lo[q]);
-                        hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
-                    }
-                    const int word0 = x.t0 / 32;
-                    for (int w = word0; w * 32 < x.t1; w++) {
-                        int klo = INT_MAX, khi = INT_MIN;
-    constexpr int U = 16 * 32 / KT;
-                                        for (int y = max(x.t0 - w * 32, 0); y < min(x.t1 - w * 32, 32); y += U) {
-                            // U tiles' loads in flight; lane l keeps tile l's range
-                            int a[U], z[U];
-#pragma unroll
-                            for (int u = 0; u < U; u++) {
-                                a[u] = INT_MAX, z[u] = INT_MIN;
-#pragma unroll
-                                for (int v = 0; v < KT / 32; v++) {
-                                    const int j = (w * 32 + y + u) * KT + v * 32 + lane;
-                                    if (j < x.kn) {
-                                        const int id = __ldg(kd + j);
-                                        a[u] = min(a[u], id);
-                                        z[u] = max(z[u], id);
-                                    }
-                                }
-                            }
-#pragma unroll
-                            for (int u = 0; u < U; u++) {
-                                const int aa = __reduce_min_sync(0xffffffffu, a[u]), zz = __reduce_max_sync(0xffffffffu, z[u]);
-                                if (lane == y + u) klo = aa, khi = zz;
-                            }
-                        }
-#pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo[q], 0) <= khi && klo <= hi[q]);
-                            const uint32_t only =
-                                __ballot_sync(0xffffffffu, lo[q] >= 0 && lo[q] == hi[q] && klo == lo[q] && khi == lo[q]);
-                            if (lane == 0) {
-                                bits[4 * (w - word0) + q] = seen;
-                                bits[4 * (w - word0) + 2 + q] = only;
-                            }
-                        }
-                    }
-                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(item_full + 8 * (turn & 1));
                 if (!more) break;
@@ -697,7 +706,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                 bool seen_here = t < before || (t >= from && t < to);
                 bool all = t < x.full && (t < x.before_whole || (t >= whole_from && t < whole_to));
                 if (bits) {
-                    const uint32_t word = bits[4 * (t / 32 - x.t0 / 32) + q], whole = bits[4 * (t / 32 - x.t0 / 32) + 2 + q];
+                    const uint32_t word = bits[4 * (t / 32 - x.word0) + q], whole = bits[4 * (t / 32 - x.word0) + 2 + q];
                     seen_here = seen_here && (word >> (t & 31) & 1);
                     all = all && (whole >> (t & 31) & 1);
                 }
