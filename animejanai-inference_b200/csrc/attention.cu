@@ -8,6 +8,7 @@
 #include <atomic>
 #include <cmath>
 
+#include "attention_few.cuh"
 #include "attention_mma.cuh"
 #include "attention_tc_run.h"
 #include "cuctx.h"
@@ -22,15 +23,16 @@ namespace {
 using namespace dev;
 
 constexpr int kSplitTiles = 4;   // at least this many key tiles a split
-constexpr int kMaxSplits = 64;
-constexpr int kTcQueries = 192;  // tcgen05 from here on (queries and keys)
+constexpr int kTcQueries = 96;  // tcgen05 from here on (queries and keys)
 
 // How an op runs, from its sizes alone (the workspace must be known before the launch).
 struct Choice {
-    bool keys = false;  // few queries: the warps share the keys out
-    bool tc = false;    // long prompts, if the tensors' layout allows: 256 queries a block on tcgen05
-    int row_tiles = 0, nsplit = 1;
-    int64_t rows = 0, blocks = 0;  // of a (sequence, key head); of the grid
+    bool few = false;   // k_attn_few, if the tensors' layout allows TMA copies
+    bool tc = false;    // k_attn_tc, likewise
+    bool keys = false;  // else k_attn_mma: few queries, the warps share the keys out
+    int pack = 0;       // k_attn_tc on copies of q, k and v with rows of this many components
+    int row_tiles = 0, key_row_tiles = 0, nsplit = 1;  // row_tiles: of 64; key_row_tiles: of 16
+    int64_t rows = 0;   // of a (sequence, key head)
     size_t space = 0;
 };
 
@@ -40,62 +42,133 @@ bool grid_reached(const ajib_attn *op)
     return op->reach_x >= op->grid_w - 1 && op->reach_y >= (std::max(op->lq, op->lk) - 1) / op->grid_w;
 }
 
-// Few queries (up to 64 rows a key head) share the keys out over warps, and over blocks until there
-// are two blocks an SM or a split has only kSplitTiles tiles.
+size_t packed_bytes(const ajib_attn *op, int dp, int tensor)
+{
+    return (size_t)op->batch * (tensor ? (size_t)op->lk * op->hk : (size_t)op->lq * op->hq) * dp * 2;
+}
+
+// Which kernel. Measured (us, 8 heads, causal; k_attn_mma / few / tc):
+//   64 components, 200 tokens 12.3 / 9.0 / 14.4, 800 26 / 18 / 27; 16 sequences of 150 20 / 23 / 14
+//   128 components, 500 tokens 27 / 14 / 19, 800 39 / 27 / 21
+// so few while all its blocks run at once, then tc; 600 windows of 144 tokens of 6 heads 303 / 723 / 169.
+// Heads of a size that TMA cannot copy (d not a multiple of 8) are copied to padded rows for tc.
+// With few queries the keys are also split until there is a block an SM or a split has only kSplitTiles
+// tiles. (us, with one / two / three blocks an SM: 2 x 16384 keys of 8 heads of 128 33 / 37 / 39, 8
+// caches of 9 to 16 thousand 78 / 79 / 75; with at least 4 / 8 tiles a split: 4000 keys 14.2 / 16.4, 1500
+// keys 12.4 / 13.9.)
 bool choose(const ajib_attn *op, Choice &c)
 {
-    const int64_t group = op->hq / op->hk;
+    const int64_t group = op->hq / op->hk, base = (int64_t)op->batch * op->hk;
     c.rows = op->lq * group;
     if (c.rows > 1 << 30) return false;
+    c.row_tiles = (int)((c.rows + 63) / 64);
+    c.key_row_tiles = (int)((c.rows + 15) / 16);
+    const int64_t few_blocks = base * c.key_row_tiles;
+    if (base * c.row_tiles > 0x7fffffff) return false;
     c.keys = c.rows <= 64;
-    if (!c.keys && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d <= 128 && op->d % 8 == 0) {
+    const int fit = sm_count() * (op->d <= 64 ? FewCfg<64>::BLOCKS : op->d <= 128 ? FewCfg<128>::BLOCKS : FewCfg<256>::BLOCKS);
+    c.few = op->lk && !op->q_doc && op->d % 8 == 0 && few_blocks <= 0x7fffffff && (c.keys || few_blocks <= fit);
+    if (!c.few && !c.keys && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d <= 128) {
         const bool grid = op->bias == AJIB_BIAS_TABLE && op->grid_w;
         c.tc = (!grid || grid_reached(op)) && (int64_t)op->batch * op->hq * ((op->lq + 255) / 256) <= 0x7fffffff &&
                (op->d <= 64 ? TcCfg<64>::smem(op) : TcCfg<128>::smem(op)) <= kMaxSmem;
-    }
-    const int bm = c.keys ? 16 : 64;
-    c.row_tiles = (int)((c.rows + bm - 1) / bm);
-    const int64_t base = (int64_t)op->batch * op->hk;
-    c.blocks = base * c.row_tiles;
-    if (c.blocks > 0x7fffffff) return false;
-    if (c.keys && c.blocks) {
-        const int tiles = (op->lk + kMmaKeys - 1) / kMmaKeys;
-        const int64_t want = (2 * sm_count() + c.blocks - 1) / c.blocks;
-        c.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, tiles / kSplitTiles), kMaxSplits));
-        if (c.nsplit > 1) {
-            c.blocks *= c.nsplit;
-            const int64_t slots = base * c.rows * c.nsplit;
-            c.space = (size_t)slots * (8 + (size_t)op->d * 4);
+        if (c.tc && op->d % 8) {
+            c.pack = (op->d + 7) / 8 * 8;
+            for (int i = 0; i < 3; i++) c.space += packed_bytes(op, c.pack, i);
         }
     }
-    return c.blocks <= 0x7fffffff;
+    if ((c.few || c.keys) && few_blocks) {
+        const int tiles = (op->lk + kMmaKeys - 1) / kMmaKeys;
+        const int64_t want = (sm_count() + few_blocks - 1) / few_blocks;
+        c.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, tiles / kSplitTiles), kMaxSplits));
+        if (few_blocks * c.nsplit > 0x7fffffff) return false;
+        if (c.nsplit > 1) c.space = (size_t)(base * c.rows * c.nsplit) * (8 + (size_t)op->d * 4);
+    }
+    return true;
 }
 
 template <typename T, int DP, bool KEYS>
-cudaError_t run_mma(const MmaDev &p, const Choice &c, cudaStream_t s)
+cudaError_t run_mma(const MmaDev &p, cudaStream_t s)
 {
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(k_attn_mma<T, DP, KEYS>, kMaxSmem, done);
     if (e != cudaSuccess) return e;
-    k_attn_mma<T, DP, KEYS><<<(unsigned)c.blocks, kMmaThreads, MmaCfg<DP, KEYS>::smem(p.a), s>>>(p);
+    const int64_t blocks = (int64_t)p.a.batch * p.a.hk * p.row_tiles * (KEYS ? p.nsplit : 1);
+    k_attn_mma<T, DP, KEYS><<<(unsigned)blocks, kMmaThreads, MmaCfg<DP, KEYS>::smem(p.a), s>>>(p);
     return cudaGetLastError();
 }
 
+template <typename T, int DP>
+cudaError_t run_few(const MmaDev &p, const CUtensorMap (&m)[3], cudaStream_t s)
+{
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(k_attn_few<T, DP>, kMaxSmem, done);
+    if (e != cudaSuccess) return e;
+    int *const err = attn_status_word();
+    if (!err) return cudaErrorUnknown;
+    const int64_t blocks = (int64_t)p.a.batch * p.a.hk * p.row_tiles * p.nsplit;
+    k_attn_few<T, DP><<<(unsigned)blocks, kFewThreads, FewCfg<DP>::SMEM, s>>>(p, m[1], m[2], err);
+    return cudaGetLastError();
+}
+
+struct PackDev {
+    const void *src[3];
+    void *dst[3];
+    int64_t sb[3], st[3], sh[3], chunks[3];  // chunks: of 8 components
+    int tokens[3], heads[3], d, width;
+};
+
+// Rows of d components copied to 16-byte aligned rows padded with zeros: a thread a chunk of 8.
+__global__ void __launch_bounds__(256) k_pack_heads(const __grid_constant__ PackDev p)
+{
+    const int x = blockIdx.y, per = (p.d + 7) / 8;
+    const uint16_t *src = (const uint16_t *)p.src[x];
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < p.chunks[x]; at += (int64_t)gridDim.x * 256) {
+        const int64_t row = at / per, bt = row / p.heads[x];
+        const int c = (int)(at - row * per) * 8, h = (int)(row - bt * p.heads[x]);
+        const int64_t b = bt / p.tokens[x];
+        const uint16_t *s = src + b * p.sb[x] + (bt - b * p.tokens[x]) * p.st[x] + h * p.sh[x] + c;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            w[i] = 0;
+            if (p.width >= 4 && c + 2 * i < p.d)
+                w[i] = __ldg(reinterpret_cast<const unsigned int *>(s + 2 * i));
+            else if (p.width < 4)
+                w[i] = (c + 2 * i < p.d ? s[2 * i] : 0u) | (c + 2 * i + 1 < p.d ? (uint32_t)s[2 * i + 1] << 16 : 0u);
+        }
+        reinterpret_cast<uint4 *>(p.dst[x])[at] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// maps: of the keys and values, where k_attn_few runs
 template <typename T>
-cudaError_t run(const MmaDev &p, const Choice &c, cudaStream_t s)
+cudaError_t run(MmaDev &p, const Choice &c, const CUtensorMap (*maps)[3], cudaStream_t s)
 {
     const int d = p.a.d;
     cudaError_t e;
-    if (c.keys)
-        e = d <= 32 ? run_mma<T, 32, true>(p, c, s) : d <= 64 ? run_mma<T, 64, true>(p, c, s)
-            : d <= 128 ? run_mma<T, 128, true>(p, c, s) : run_mma<T, 256, true>(p, c, s);
+    p.row_tiles = maps || c.keys ? c.key_row_tiles : c.row_tiles;
+    p.nsplit = maps || c.keys ? c.nsplit : 1;
+    if (maps)
+        e = d <= 64 ? run_few<T, 64>(p, *maps, s) : d <= 128 ? run_few<T, 128>(p, *maps, s) : run_few<T, 256>(p, *maps, s);
+    else if (c.keys)
+        e = d <= 32 ? run_mma<T, 32, true>(p, s) : d <= 64 ? run_mma<T, 64, true>(p, s)
+            : d <= 128 ? run_mma<T, 128, true>(p, s) : run_mma<T, 256, true>(p, s);
     else
-        e = d <= 32 ? run_mma<T, 32, false>(p, c, s) : d <= 64 ? run_mma<T, 64, false>(p, c, s)
-            : d <= 128 ? run_mma<T, 128, false>(p, c, s) : run_mma<T, 256, false>(p, c, s);
-    if (e != cudaSuccess || c.nsplit == 1) return e;
+        e = d <= 32 ? run_mma<T, 32, false>(p, s) : d <= 64 ? run_mma<T, 64, false>(p, s)
+            : d <= 128 ? run_mma<T, 128, false>(p, s) : run_mma<T, 256, false>(p, s);
+    if (e != cudaSuccess || p.nsplit == 1) return e;
     const int64_t rows = (int64_t)p.a.batch * p.a.hk * p.rows;
-    k_attn_join<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_attn_join<T>, p);
 }
 
 // A tensor map of tiles of `rows` tokens, 64 components of one head (128-byte swizzle; zeros outside).
@@ -231,8 +304,6 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
     p.reach_x = op->reach_x;
     p.masked = p.left != far || p.right != far || p.q_doc;
     m.rows = (int)c.rows;
-    m.row_tiles = c.row_tiles;
-    m.nsplit = c.nsplit;
     m.wq = heads_width(q, b, op->lq, op->hq, d);
     m.wo = heads_width(out, b, op->lq, op->hq, d);
     m.wkv = op->lk ? std::min(heads_width(k, b, op->lk, op->hk, d), heads_width(v, b, op->lk, op->hk, d)) : 16;
@@ -245,8 +316,33 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
     }
     CUtensorMap maps[3];
     const int key_tile = d <= 64 ? TcCfg<64>::KT : TcCfg<128>::KT;
-    if (c.tc && map_of(&maps[0], q, b, op->lq, op->hq, d, op->dtype, 128) && map_of(&maps[1], k, b, op->lk, op->hk, d, op->dtype, key_tile) &&
-        map_of(&maps[2], v, b, op->lk, op->hk, d, op->dtype, key_tile)) {
+    ajib_heads packed[3] = {*q, op->lk ? *k : *q, op->lk ? *v : *q};
+    if (c.pack) {
+        PackDev w{};
+        char *to = (char *)workspace;
+        int64_t most = 0;
+        for (int i = 0; i < 3; i++) {
+            w.src[i] = packed[i].p;
+            w.dst[i] = to;
+            w.sb[i] = packed[i].sb, w.st[i] = packed[i].st, w.sh[i] = packed[i].sh;
+            w.tokens[i] = i ? op->lk : op->lq;
+            w.heads[i] = i ? op->hk : op->hq;
+            w.chunks[i] = (int64_t)b * w.tokens[i] * w.heads[i] * (c.pack / 8);
+            most = std::max(most, w.chunks[i]);
+            const int64_t row = (int64_t)w.heads[i] * c.pack;
+            packed[i] = {to, row * w.tokens[i], row, c.pack};
+            to += packed_bytes(op, c.pack, i);
+        }
+        w.d = d;
+        w.width = std::min(m.wq, m.wkv);
+        const unsigned blocks = (unsigned)std::min<int64_t>((most + 255) / 256, 16 * sm_count());
+        k_pack_heads<<<dim3(blocks, 3), 256, 0, (cudaStream_t)stream>>>(w);
+        if (cudaGetLastError() != cudaSuccess) return AJIB_ERR_CUDA;
+    }
+    const int md = c.pack ? c.pack : d;
+    if (c.tc && map_of(&maps[0], &packed[0], b, op->lq, op->hq, md, op->dtype, 128) &&
+        map_of(&maps[1], &packed[1], b, op->lk, op->hk, md, op->dtype, key_tile) &&
+        map_of(&maps[2], &packed[2], b, op->lk, op->hk, md, op->dtype, key_tile)) {
         TcDev t{};
         t.a = p;
         t.tiles = (op->lq + 255) / 256;
@@ -263,7 +359,10 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
                                                     : attn_tc_bf16(t, op, maps, (cudaStream_t)stream);
         return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
     }
-    const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(m, c, (cudaStream_t)stream)
-                                                : run<__nv_bfloat16>(m, c, (cudaStream_t)stream);
+    m.plain = m.bias_form == kBiasNone && !(op->cap > 0);
+    const bool few = c.few && map_of(&maps[1], k, b, op->lk, op->hk, d, op->dtype, kMmaKeys) &&
+                     map_of(&maps[2], v, b, op->lk, op->hk, d, op->dtype, kMmaKeys);
+    const cudaError_t e = op->dtype == AJIB_F16 ? run<__half>(m, c, few ? &maps : nullptr, (cudaStream_t)stream)
+                                                : run<__nv_bfloat16>(m, c, few ? &maps : nullptr, (cudaStream_t)stream);
     return e == cudaSuccess ? AJIB_OK : AJIB_ERR_CUDA;
 }

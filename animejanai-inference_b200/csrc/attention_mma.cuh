@@ -27,6 +27,7 @@ struct MmaDev {
     AttnDev a;
     int rows, row_tiles, nsplit;  // rows = lq * group of a (sequence, key head)
     int bias_form;
+    int plain;        // scores are the scaled products alone
     int wq, wkv, wo;  // widest copies (bytes) of q, of k and v, of out
     float *part;      // [sequence, key head, row][nsplit][d] unnormalised outputs
     float2 *part_ml;  // [..][nsplit] maximum (base 2) and sum
@@ -34,6 +35,38 @@ struct MmaDev {
 
 namespace dev {
 
+// mbar_wait with a hint (10 us) of how long the hardware may keep a waiting thread asleep: the roles of
+// this kernel wait for one another most of the time, and polling took their issue slots.
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err, int code)
+{
+    if (mbar_test_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer();
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(10000u)
+            : "memory");
+        if (done) return true;
+        if (globaltimer() - t0 > 2000000000ull) {
+            atomicCAS(err, 0, code);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool tc_wait_warp(uint32_t bar, uint32_t parity, int *err, int code)
+{
+    return __all_sync(0xffffffffu, tc_wait(bar, parity, err, code));
+}
+// One lane of a converged warp. (Told by a lane number instead, the compiler takes the operands of the
+// branch's products and copies for divergent, and each issue costs 140 cycles instead of a few.)
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+    return r != 0;
+}
 template <typename T> struct MmaOp;
 template <> struct MmaOp<__half> {
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -161,6 +194,69 @@ template <int DP, bool KEYS> struct MmaCfg {
         return BITS + words * 8;
     }
 };
+
+// Joins the results of four warps (threads 0 to 127) over keys of their own for the same 16 rows, in
+// memory of 4 * 16 * (DP + 2) floats, and writes them out, or to the workspace where the keys are
+// split. Rows that are not finite are taken again from the keys [j_begin, j_end) that they see.
+template <typename T, int DP>
+__device__ __forceinline__ void join_warps(const MmaDev &P, int b, int hk, int row0, int rows, int split, int qn, int kn,
+                                           int j_begin, int j_end, const float (&o)[DP / 8][4], const float (&m)[2],
+                                           const float (&l)[2], float *memory, float *scratch)
+{
+    const AttnDev &p = P.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float *const jm = memory, *const jl = jm + 64, *const jo = jl + 64;  // [warp][16], [warp][16], [warp][16][DP]
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int r = (lane >> 2) + 8 * x;
+        if ((lane & 3) == 0) {
+            jm[warp * 16 + r] = m[x];
+            jl[warp * 16 + r] = l[x];
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++)
+            *reinterpret_cast<float2 *>(jo + (warp * 16 + r) * DP + n * 8 + 2 * (lane & 3)) =
+                make_float2(o[n][2 * x], o[n][2 * x + 1]);
+    }
+    named_bar_sync(1, 128);
+    for (int r = warp; r < 16 && row0 + r < rows; r += 4) {
+        const int row = row0 + r, i = row / p.group, h = hk * p.group + row - i * p.group;
+        float top = -INFINITY, sum = 0.f, ro[8], f[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = fmaxf(top, jm[w * 16 + r]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[w] = exp2_fast(jm[w * 16 + r] - (top == -INFINITY ? 0.f : top));
+            sum += jl[w * 16 + r] * f[w];
+        }
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int c = lane + 32 * e;
+            ro[e] = 0.f;
+            if (c < p.d) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) ro[e] += jo[(w * 16 + r) * DP + c] * f[w];
+                odd |= !(fabsf(ro[e]) < INFINITY);
+            }
+        }
+        if (p.masked && __any_sync(0xffffffffu, odd))
+            attend_row<T>(p, b, h, i, qn, kn, j_begin, j_end, scratch, top, sum, ro);
+        if (P.nsplit > 1) {
+            const int64_t slot = (((int64_t)b * p.hk + hk) * P.rows + row) * P.nsplit + split;
+            if (lane == 0) P.part_ml[slot] = make_float2(top, sum);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (lane + 32 * e < p.d) P.part[slot * p.d + lane + 32 * e] = ro[e];
+        } else {
+            T *dst = (T *)p.out + b * p.ob + i * p.ot + h * p.oh;
+            const float g = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (lane + 32 * e < p.d) dst[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : ro[e] * g);
+        }
+    }
+}
 
 template <typename T, int DP, bool KEYS>
 __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant__ MmaDev P)
@@ -526,90 +622,48 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
 
     // ---- KEYS: join the four warps, then finish or hand on this split ----
     __syncthreads();
-    float *const jm = (float *)stage0, *const jl = jm + 64, *const jo = jl + 64;  // [warp][16], [warp][16], [warp][16][DP]
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int r = (lane >> 2) + 8 * x;
-        if ((lane & 3) == 0) {
-            jm[warp * 16 + r] = m[x];
-            jl[warp * 16 + r] = l[x];
-        }
-#pragma unroll
-        for (int n = 0; n < DP / 8; n++)
-            *reinterpret_cast<float2 *>(jo + (warp * 16 + r) * DP + n * 8 + 2 * (lane & 3)) =
-                make_float2(o[n][2 * x], o[n][2 * x + 1]);
-    }
-    __syncthreads();
-    for (int r = warp; r < 16 && row0 + r < rows; r += 4) {
-        const int row = row0 + r, i = row / p.group, h = hk * p.group + row - i * p.group;
-        float top = -INFINITY, sum = 0.f, ro[8], f[4];
-#pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, jm[w * 16 + r]);
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            f[w] = exp2_fast(jm[w * 16 + r] - (top == -INFINITY ? 0.f : top));
-            sum += jl[w * 16 + r] * f[w];
-        }
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int c = lane + 32 * e;
-            ro[e] = 0.f;
-            if (c < p.d) {
-#pragma unroll
-                for (int w = 0; w < 4; w++) ro[e] += jo[(w * 16 + r) * DP + c] * f[w];
-                odd |= !(fabsf(ro[e]) < INFINITY);
-            }
-        }
-        if (p.masked && __any_sync(0xffffffffu, odd))
-            attend_row<T>(p, b, h, i, qn, kn, j_begin, j_end, scratch, top, sum, ro);
-        if (P.nsplit > 1) {
-            const int64_t slot = (((int64_t)b * p.hk + hk) * P.rows + row) * P.nsplit + split;
-            if (lane == 0) P.part_ml[slot] = make_float2(top, sum);
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (lane + 32 * e < p.d) P.part[slot * p.d + lane + 32 * e] = ro[e];
-        } else {
-            T *dst = (T *)p.out + b * p.ob + i * p.ot + h * p.oh;
-            const float g = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (lane + 32 * e < p.d) dst[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : ro[e] * g);
-        }
-    }
+    join_warps<T, DP>(P, b, hk, row0, rows, split, qn, kn, j_begin, j_end, o, m, l, (float *)stage0, scratch);
 }
 
-// Joins the splits: one warp a row.
+constexpr int kMaxSplits = 128;
+
+// Joins the splits, always in the same order: a block a row, whose warps take every fourth split each
+// with four of them in flight.
 template <typename T>
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ MmaDev P)
 {
+    __shared__ float f[kMaxSplits], wm[4], wl[4], wo[4][256];
     const AttnDev &p = P.a;
-    const int lane = threadIdx.x & 31;
-    const int64_t row_at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row_at >= (int64_t)p.batch * p.hk * P.rows) return;
-    const int64_t bh = row_at / P.rows;
-    const int row = (int)(row_at - bh * P.rows), b = (int)(bh / p.hk), hk = (int)(bh - (int64_t)b * p.hk);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t bh = blockIdx.x / P.rows;
+    const int row = (int)(blockIdx.x - bh * P.rows), b = bh / p.hk, hk = (int)(bh - (uint32_t)b * p.hk);
     const int i = row / p.group, h = hk * p.group + row - i * p.group;
+    const int64_t slot = (int64_t)blockIdx.x * P.nsplit;
     if (i >= q_count(p, b)) return;
-    float top = -INFINITY, sum = 0.f, ro[8];
-    for (int s = 0; s < P.nsplit; s++) top = fmaxf(top, P.part_ml[row_at * P.nsplit + s].x);
-    const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int e = 0; e < 8; e++) ro[e] = 0.f;
-    for (int s = 0; s < P.nsplit; s++) {
-        const float2 ml = P.part_ml[row_at * P.nsplit + s];
-        const float f = exp2_fast(ml.x - base);
-        sum += ml.y * f;
-        const float *src = P.part + (row_at * P.nsplit + s) * p.d;
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (lane + 32 * e < p.d) ro[e] += src[lane + 32 * e] * f;
+    griddep_wait();  // launched while the splits may still run
+    const float2 ml = tid < P.nsplit ? P.part_ml[slot + tid] : make_float2(-INFINITY, 0.f);
+    float top = ml.x;
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    if (lane == 0) wm[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    f[tid] = exp2_fast(ml.x - (top == -INFINITY ? 0.f : top));
+    float sum = ml.y * f[tid];
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) wl[warp] = sum;
+    __syncthreads();
+    sum = (wl[0] + wl[1]) + (wl[2] + wl[3]);
+    for (int c = lane; c < p.d; c += 32) {
+        float a = 0.f;
+#pragma unroll 4
+        for (int s = warp; s < P.nsplit; s += 4) a = fmaf(P.part[(slot + s) * p.d + c], f[s], a);
+        wo[warp][c] = a;
     }
+    __syncthreads();
     T *dst = (T *)p.out + b * p.ob + i * p.ot + h * p.oh;
     const float g = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-        if (lane + 32 * e < p.d) dst[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : ro[e] * g);
+    for (int c = tid; c < p.d; c += 128)
+        dst[c] = from_f<T>(sum == 0.f ? 0.f : ((wo[0][c] + wo[1][c]) + (wo[2][c] + wo[3][c])) * g);
 }
 
 }  // namespace dev

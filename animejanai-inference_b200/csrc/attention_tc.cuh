@@ -101,38 +101,6 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_of(int N, boo
     return (1u << 4) | (type << 7) | (type << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
 }
-// mbar_wait with a hint (10 us) of how long the hardware may keep a waiting thread asleep: the roles of
-// this kernel wait for one another most of the time, and polling took their issue slots.
-__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err, int code)
-{
-    if (mbar_test_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
-    for (;;) {
-        uint32_t done;
-        asm volatile(
-            "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity), "r"(10000u)
-            : "memory");
-        if (done) return true;
-        if (globaltimer() - t0 > 2000000000ull) {
-            atomicCAS(err, 0, code);
-            return false;
-        }
-    }
-}
-__device__ __forceinline__ bool tc_wait_warp(uint32_t bar, uint32_t parity, int *err, int code)
-{
-    return __all_sync(0xffffffffu, tc_wait(bar, parity, err, code));
-}
-// One lane of a converged warp. (Told by a lane number instead, the compiler takes the operands of the
-// branch's products and copies for divergent, and each issue costs 140 cycles instead of a few.)
-__device__ __forceinline__ bool elect_one()
-{
-    uint32_t r;
-    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
-    return r != 0;
-}
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
@@ -932,7 +900,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                     w[y] = MmaOp<T>::pack(o[2 * y], o[2 * y + 1]);
                 }
                 if (!there) continue;
-                // (d is a multiple of 8, of 16 where 32-byte stores are allowed)
+                // (d is a multiple of what a store holds)
                 if (P.wo == 32) {
 #pragma unroll
                     for (int y = 0; y < 2; y++)
@@ -947,6 +915,10 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                         if (c + 8 * y < p.d)
                             *reinterpret_cast<uint4 *>(dst + c + 8 * y) =
                                 make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
+                } else if (P.wo == 4) {
+#pragma unroll
+                    for (int y = 0; y < 16; y++)
+                        if (c + 2 * y < p.d) *reinterpret_cast<uint32_t *>(dst + c + 2 * y) = w[y];
                 } else {
 #pragma unroll
                     for (int y = 0; y < 32; y++)
