@@ -59,7 +59,7 @@ template <int DP> struct TcCfg {
     static constexpr int QTILE = 128 * DP * 2, TILE = KT * DP * 2, HALF = KT * 128;  // HALF: a tile's 64 components
     static constexpr int Q = 0, K = 2 * QTILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
     static constexpr int BARS = SCRATCH + 8 * 256 * 4;  // attend_row's queries, a warp each
-    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 8 + 4;
+    static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 4;
     static constexpr int COLUMNS = 2 * KT + 2 * DP;     // of TMEM: scores of both query tiles, then outputs
     // One block of 384 threads an SM: 168 registers, of which the softmax warps take 216 and the others 72.
     // Two blocks: 80 each.
@@ -160,23 +160,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
-// 2^x of two, on the FMA pipe: x = i + f with i whole and f in [-1/2, 1/2] (adding 1.5 * 2^23 rounds x to
-// i in the low bits), 2^f by a polynomial (minimax fit of degree 4, relative error 2.7e-6: 1/180 of
-// fp16's half step, to which the result is rounded), times 2^i; 0 below 2^-126.5 (i = -127 has no bits left), -inf included. NaN stays NaN.
-__device__ __forceinline__ F2 f2_exp2(float a, float b)
-{
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
-    const F2 x = f2(a, b), magic = f2(12582912.f, 12582912.f);
-    const F2 r = f2_add(x, magic), f = f2_add(x, f2_fma(r, f2(-1.f, -1.f), magic));
-    F2 y = f2_fma(f2(0.009567738510668278f, 0.009567738510668278f), f, f2(0.05591749772429466f, 0.05591749772429466f));
-    y = f2_fma(y, f, f2(0.24024811387062073f, 0.24024811387062073f));
-    y = f2_fma(y, f, f2(0.6931219100952148f, 0.6931219100952148f));
-    y = f2_fma(y, f, f2(0.9999992251396179f, 0.9999992251396179f));
-    float ra, rb;
-    f2_out(r, ra, rb);
-    return f2_mul(y, f2(__int_as_float((__float_as_int(ra) << 23) + 0x3f800000), __int_as_float((__float_as_int(rb) << 23) + 0x3f800000)));
-}
 // tanh of two in [-1, 1] on the FMA pipe: odd polynomial of degree 11 (minimax fit, error 3e-7).
 __device__ __forceinline__ F2 f2_tanh(F2 x)
 {
@@ -391,8 +374,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
     const uint32_t q_full = bars, q_empty = q_full + 16, k_full = q_empty + 16, k_empty = k_full + 8 * C::ST,
                    v_full = k_empty + 8 * C::ST, v_empty = v_full + 8 * C::ST, s_full = v_empty + 8 * C::ST,
                    p_full = s_full + 16, o_full = p_full + 16,
-                   item_full = o_full + 16, item_empty = item_full + 16, go = item_empty + 16,
-                   p_half = go + 64, meet = p_half + 16;
+                   item_full = o_full + 16, item_empty = item_full + 16,
+                   p_half = item_empty + 16, meet = p_half + 16;
     uint32_t *const tmem_at = (uint32_t *)(sm + C::BARS + C::NBAR * 8);
     TcItem *const items = (TcItem *)(sm + C::ITEMS);
     static_assert(sizeof(TcItem) <= 128, "");
@@ -405,7 +388,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
         tma_prefetch_desc(&mk);
         tma_prefetch_desc(&mv);
         for (uint32_t x = bars; x < meet + 16; x += 8)
-            mbar_init(x, x >= p_half ? 4 : x >= go ? 1 : x >= item_empty ? 11 : x >= item_full ? 1 : x >= p_full && x < o_full ? 4 : x >= k_empty && x < v_full || x >= v_empty && x < s_full ? 2 : 1);
+            mbar_init(x, x >= p_half ? 4 : x >= item_empty ? 11 : x >= item_full ? 1 : x >= p_full && x < o_full ? 4 : x >= k_empty && x < v_full || x >= v_empty && x < s_full ? 2 : 1);
         fence_mbar_init();
     }
     tc_fence_before();
@@ -628,7 +611,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
             named_bar_sync(3, 256);
         }
         // Two blocks an SM: 80 registers hold 32 scores of a row at a time, read twice. One: the whole row.
-        constexpr bool TWICE = C::BLOCKS == 2, TURNS = C::BLOCKS == 1;
+        constexpr bool TWICE = C::BLOCKS == 2;
         constexpr int CH = 32, W = TWICE ? 32 : KT;
         uint32_t s_phase = 0, o_phase = 0;
         uint32_t meets = 0;
@@ -636,18 +619,6 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
             __syncwarp();
             if (lane == 0) mbar_arrive(meet + 8 * q);
             return tc_wait_warp(meet + 8 * q, meets++ & 1, P.err, 219);
-        };
-        // Warps w and w + 4 share a scheduler and its exponential unit (4 a cycle): they take turns, so that
-        // one's exponentials run beside the other's products, loads and maxima and not beside its exponentials.
-        uint32_t turns = q ? 0 : 1;
-        auto my_turn = [&]() {
-            const bool done = tc_wait_warp(go + 8 * warp, turns & 1, P.err, 217);
-            turns++;
-            return done;
-        };
-        auto pass_turn = [&]() {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(go + 8 * (warp ^ 4));
         };
         for (; __all_sync(0xffffffffu, next()); turn++) {
             if (grid && table_h != x.h) {
@@ -678,14 +649,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                     seen_here = seen_here && (word >> (t & 31) & 1);
                     all = all && (whole >> (t & 31) & 1);
                 }
-                if (!seen_here) {
-                    // the other query tile's alone: pass its turn on
-                    if (TURNS && x.both && tc_active(x, bits, 1 - q, t)) {
-                        if (!(ok = my_turn())) break;
-                        pass_turn();
-                    }
-                    continue;
-                }
+                if (!seen_here) continue;
                 const int j0 = t * KT;
                 if (!(ok = tc_wait_warp(s_full + 8 * q, s_phase, P.err, 210))) break;
                 s_phase ^= 1;
@@ -824,20 +788,13 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                     }
 #pragma unroll
                     for (int c = 0; c < W; c += 2) f2_out(f2_fma(f2(s[c], s[c + 1]), sc2, base2), s[c], s[c + 1]);
-                    if (TURNS && x.both && !(ok = my_turn())) break;
 #pragma unroll
                     for (int c = 0; c < W; c += 32) {
                         uint32_t w[16];
 #pragma unroll
                         for (int y = 0; y < 16; y++) {
-                            F2 e;
-                            if (!TWICE && y % 4 == 3)  // a quarter of them on the FMA pipe
-                                e = f2_exp2(s[c + 2 * y], s[c + 2 * y + 1]);
-                            else
-                                e = f2(exp2_fast(s[c + 2 * y]), exp2_fast(s[c + 2 * y + 1]));
-                            sum[y & 1] = f2_add(sum[y & 1], e);
-                            float a, z;
-                            f2_out(e, a, z);
+                            const float a = exp2_fast(s[c + 2 * y]), z = exp2_fast(s[c + 2 * y + 1]);
+                            sum[y & 1] = f2_add(sum[y & 1], f2(a, z));
                             w[y] = MmaOp<T>::pack(a, z);
                         }
                         tmem_st16(s_at + (c0 + c) / 2, w);
@@ -849,9 +806,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                             if (lane == 0) mbar_arrive(p_half + 8 * q);
                         }
                     }
-                    if (TURNS && x.both) pass_turn();
                 }
-                if (!ok) break;
                 float la, lb;
                 f2_out(f2_add(sum[0], sum[1]), la, lb);
                 l += la + lb;
