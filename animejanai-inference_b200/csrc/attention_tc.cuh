@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "attention_mma.cuh"
+#include "f32x2.cuh"
 
 namespace ajib {
 
@@ -124,35 +125,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v)
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// Two fp32 operations an instruction.
-struct F2 {
-    uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float a, float b)
-{
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f2_out(F2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c)
-{
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b)
-{
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b)
-{
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float r;

@@ -20,6 +20,7 @@
 #include <cmath>
 #include <new>
 
+#include "f32x2.cuh"
 #include "heads.h"
 
 struct ajib_rotary {
@@ -57,23 +58,27 @@ template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// cos and sin of pair i (of npair) at a position, times the amplitude.
-__device__ __forceinline__ void pair_angle(const QkDev &p, int position, int i, float &c, float &s)
+// What a position's pairs turn by: itself, or its row and column.
+struct Place {
+    int64_t row, column;
+};
+__device__ __forceinline__ Place place_of(const QkDev &p, int position)
 {
-    int64_t at = position;
-    if (p.axes == 2) {
-        int row = position / p.grid_w;
-        if (position - row * p.grid_w < 0) row--;
-        const int per = p.rot >> 2;
-        if (i < per) {
-            at = row;
-        } else {
-            at = position - (int64_t)row * p.grid_w;
-            i -= per;
-        }
-    }
-    const uint64_t turn = (uint64_t)at * p.turns[i];
-    sincospif((float)(int)(turn >> 32) * 0x1p-31f, &s, &c);
+    if (p.axes != 2) return {position, position};
+    int row = position / p.grid_w;
+    if (position - row * p.grid_w < 0) row--;
+    return {row, position - (int64_t)row * p.grid_w};
+}
+
+// cos and sin of pair i, times the amplitude. The angle is within half a turn of zero, where the
+// hardware's sine and cosine are good to 2^-20.9: 1/1000 of fp16's half step.
+__device__ __forceinline__ void pair_angle(const QkDev &p, const Place &at, int i, float &c, float &s)
+{
+    const int per = p.axes == 2 ? p.rot >> 2 : p.rot >> 1;
+    const uint64_t turn = (uint64_t)(i < per ? at.row : at.column) * p.turns[i < per ? i : i - per];
+    const float x = (float)(int)(turn >> 32) * (3.14159265358979f * 0x1p-31f);
+    asm("cos.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(x));
+    asm("sin.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(x));
     c *= p.amplitude;
     s *= p.amplitude;
 }
@@ -130,7 +135,8 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ Q
         }
         f = norm_factor(p, sum, scale);
     }
-    const int npair = p.rot >> 1, position = p.rot ? position_of(p, b, t) : 0;
+    const int npair = p.rot >> 1;
+    const Place place = place_of(p, p.rot ? position_of(p, b, t) : 0);
     for (int i = lane; i < npair; i += 32) {
         const int i1 = p.interleaved ? 2 * i : i, i2 = p.interleaved ? 2 * i + 1 : i + npair;
         float x1 = to_f(src[i1]) * f, x2 = to_f(src[i2]) * f, c, s;
@@ -138,7 +144,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ Q
             x1 *= x.w[i1];
             x2 *= x.w[i2];
         }
-        pair_angle(p, position, i, c, s);
+        pair_angle(p, place, i, c, s);
         dst[i1] = from_f<T>(x1 * c - x2 * s);
         dst[i2] = from_f<T>(x2 * c + x1 * s);
     }
@@ -170,6 +176,42 @@ template <> struct Pair<__nv_bfloat16> {
     }
 };
 
+using dev::F2;
+using dev::f2;
+using dev::f2_add;
+using dev::f2_fma;
+using dev::f2_mul;
+using dev::f2_out;
+
+// The sum of the squares of a lane's 16 components times scale.
+__device__ __forceinline__ float sum_squares(const F2 (&a)[4], const F2 (&e)[4], float scale)
+{
+    const F2 by = f2(scale, scale);
+    F2 sum = f2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const F2 x = f2_mul(a[i], by), y = f2_mul(e[i], by);
+        sum = f2_fma(x, x, f2_fma(y, y, sum));
+    }
+    float lo, hi;
+    f2_out(sum, lo, hi);
+    return lo + hi;
+}
+
+enum { kTurnNone = 0, kTurnHalf = 1, kTurnInterleaved = 2 };
+
+template <typename T> __device__ __forceinline__ uint4 pack8(const F2 (&x)[4])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float lo, hi;
+        f2_out(x[i], lo, hi);
+        w[i] = Pair<T>::pack(lo, hi);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // d and the turned components multiples of 16, every row 16-byte aligned: a lane holds two chunks of 8
 // components of a head (16-byte loads, neighbouring lanes on neighbouring chunks), GP lanes (a power of
 // two, d / 16 of them at work) a head. HALF: chunk g of the turned components' first half and of their
@@ -177,8 +219,8 @@ template <> struct Pair<__nv_bfloat16> {
 // its 8 angles once and walks the heads of its token, `split` groups to a token so that small batches
 // fill the machine too. U heads are in flight at a time: DRAM latency times bandwidth is some 45 KB an
 // SM, four blocks of 256 lanes with 64 bytes each hold 64 KB.
-template <typename T, int GP, bool NORM, bool TURN>
-__global__ void __launch_bounds__(kQkThreads, NORM && TURN ? 3 : 4) k_qk_vec(const __grid_constant__ QkDev p)
+template <typename T, int GP, bool NORM, int TURN>
+__global__ void __launch_bounds__(kQkThreads, TURN ? 3 : 4) k_qk_vec(const __grid_constant__ QkDev p)
 {
     const uint32_t slot = blockIdx.x * (kQkThreads / GP) + threadIdx.x / GP;  // (below 2^32: run_qk)
     const int g = threadIdx.x % GP;
@@ -189,36 +231,49 @@ __global__ void __launch_bounds__(kQkThreads, NORM && TURN ? 3 : 4) k_qk_vec(con
     const int b = (int)(bt / p.tokens), t = (int)(bt - (uint32_t)b * p.tokens);
     // lanes of a warp stay together for the sums: what a lane has no part in, it neither reads nor writes
     const bool live = there && g * 16 < p.d && !(p.len && t >= p.len[b]);
-    const bool apart = TURN && !p.interleaved;
+    constexpr bool apart = TURN == kTurnHalf;
     int c1 = 8 * g, c2 = (p.d >> 1) + 8 * g;
     if (apart) {
         const int turned = p.rot >> 4, rest = (p.d - p.rot) >> 1;  // lanes at work on each part
         c1 = g < turned ? 8 * g : p.rot + 8 * (g - turned);
         c2 = c1 + (g < turned ? p.rot >> 1 : rest);
     }
-    float c[8], s[8];
+    // HALF: c, s, sn = cos, sin, -sin of the chunk's pairs; INTERLEAVED: c, sn = (cos, cos), (-sin, sin) of
+    // the first chunk's pairs and s, ce the same of the second's
+    F2 c[4], s[4], sn[4], ce[4];
     if (TURN) {
+        float co[8], si[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) c[i] = 1.f, s[i] = 0.f;
+        for (int i = 0; i < 8; i++) co[i] = 1.f, si[i] = 0.f;
         if (live && c1 < p.rot) {
-            const int position = position_of(p, b, t);
+            const Place place = place_of(p, position_of(p, b, t));
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int pair = apart ? c1 + i : (i < 4 ? c1 >> 1 : (c2 >> 1) - 4) + i;
-                if (2 * pair < p.rot) pair_angle(p, position, pair, c[i], s[i]);
+                if (2 * pair < p.rot) pair_angle(p, place, pair, co[i], si[i]);
             }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c[i] = apart ? f2(co[2 * i], co[2 * i + 1]) : f2(co[i], co[i]);
+            s[i] = apart ? f2(si[2 * i], si[2 * i + 1]) : f2(co[4 + i], co[4 + i]);
+            sn[i] = apart ? f2(-si[2 * i], -si[2 * i + 1]) : f2(-si[i], si[i]);
+            ce[i] = f2(-si[4 + i], si[4 + i]);
         }
     }
     const unsigned all = ((1u << GP) - 1) << (threadIdx.x % 32 / GP * GP);
     int h = h0;
     for (int part = 0; part < 2; part++) {
         const QkTensor &q = p.t[part];
-        float w1[8], w2[8];
+        F2 w1[4], w2[4];
         if (NORM) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                w1[i] = live && q.w ? __ldg(q.w + c1 + i) : 1.f;
-                w2[i] = live && q.w ? __ldg(q.w + c2 + i) : 1.f;
+            for (int i = 0; i < 4; i++) {
+                w1[i] = w2[i] = f2(1.f, 1.f);
+                if (live && q.w) {
+                    w1[i] = f2(__ldg(q.w + c1 + 2 * i), __ldg(q.w + c1 + 2 * i + 1));
+                    w2[i] = f2(__ldg(q.w + c2 + 2 * i), __ldg(q.w + c2 + 2 * i + 1));
+                }
             }
         }
         const T *src = (const T *)q.src + b * q.sb + t * q.st + h * q.sh;
@@ -237,60 +292,54 @@ __global__ void __launch_bounds__(kQkThreads, NORM && TURN ? 3 : 4) k_qk_vec(con
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                float a[8], e[8];
+                F2 a[4], e[4];
                 const uint32_t *xa = &x[u][0].x, *xe = &x[u][1].x;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float2 fa = Pair<T>::unpack(xa[i]), fe = Pair<T>::unpack(xe[i]);
-                    a[2 * i] = fa.x, a[2 * i + 1] = fa.y;
-                    e[2 * i] = fe.x, e[2 * i + 1] = fe.y;
+                    a[i] = f2(fa.x, fa.y);
+                    e[i] = f2(fe.x, fe.y);
                 }
                 if (NORM) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sum = fmaf(a[i], a[i], fmaf(e[i], e[i], sum));
+                    float sum = sum_squares(a, e, 1.f);
 #pragma unroll
                     for (int m = GP / 2; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
                     const float scale = rescale_of(p, sum);
                     if (scale != 1.f) {  // (every lane of the head agrees)
-                        sum = 0.f;
-                        for (int i = 0; i < 8; i++)
-                            sum += (a[i] * scale) * (a[i] * scale) + (e[i] * scale) * (e[i] * scale);
+                        sum = sum_squares(a, e, scale);
                         for (int m = GP / 2; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
                     }
                     const float f = norm_factor(p, sum, scale);
+                    const F2 ff = f2(f, f);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        a[i] = a[i] * f * w1[i];
-                        e[i] = e[i] * f * w2[i];
+                    for (int i = 0; i < 4; i++) {
+                        a[i] = f2_mul(f2_mul(a[i], ff), w1[i]);
+                        e[i] = f2_mul(f2_mul(e[i], ff), w2[i]);
                     }
                 }
                 if (TURN) {  // (what does not turn has angle 0)
                     if (apart) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float x1 = a[i], x2 = e[i];
-                            a[i] = x1 * c[i] - x2 * s[i];
-                            e[i] = x2 * c[i] + x1 * s[i];
+                        for (int i = 0; i < 4; i++) {
+                            const F2 x1 = a[i], x2 = e[i];
+                            a[i] = f2_fma(x1, c[i], f2_mul(x2, sn[i]));
+                            e[i] = f2_fma(x2, c[i], f2_mul(x1, s[i]));
                         }
                     } else {
+                        // a chunk is x1, x2 pairs: c holds an angle twice, sn its sine as -s, s
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const float x1 = a[2 * i], x2 = a[2 * i + 1], y1 = e[2 * i], y2 = e[2 * i + 1];
-                            a[2 * i] = x1 * c[i] - x2 * s[i];
-                            a[2 * i + 1] = x2 * c[i] + x1 * s[i];
-                            e[2 * i] = y1 * c[4 + i] - y2 * s[4 + i];
-                            e[2 * i + 1] = y2 * c[4 + i] + y1 * s[4 + i];
+                            float x1, x2, y1, y2;
+                            f2_out(a[i], x1, x2);
+                            f2_out(e[i], y1, y2);
+                            a[i] = f2_fma(a[i], c[i], f2_mul(f2(x2, x1), sn[i]));
+                            e[i] = f2_fma(e[i], s[i], f2_mul(f2(y2, y1), ce[i]));
                         }
                     }
                 }
                 if (live && h + u * p.split < q.heads) {
-                    *reinterpret_cast<uint4 *>(dst + u * out_step + c1) =
-                        make_uint4(Pair<T>::pack(a[0], a[1]), Pair<T>::pack(a[2], a[3]), Pair<T>::pack(a[4], a[5]),
-                                   Pair<T>::pack(a[6], a[7]));
-                    *reinterpret_cast<uint4 *>(dst + u * out_step + c2) =
-                        make_uint4(Pair<T>::pack(e[0], e[1]), Pair<T>::pack(e[2], e[3]), Pair<T>::pack(e[4], e[5]),
-                                   Pair<T>::pack(e[6], e[7]));
+                    *reinterpret_cast<uint4 *>(dst + u * out_step + c1) = pack8<T>(a);
+                    *reinterpret_cast<uint4 *>(dst + u * out_step + c2) = pack8<T>(e);
                 }
             }
             src += U * step;
@@ -307,12 +356,16 @@ cudaError_t run_vec(const QkDev &p, cudaStream_t s)
     const int64_t blocks = (p.slots * GP + kQkThreads - 1) / kQkThreads;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const unsigned n = (unsigned)blocks;
-    if (p.norm && p.rot)
-        k_qk_vec<T, GP, true, true><<<n, kQkThreads, 0, s>>>(p);
+    if (!p.rot)
+        k_qk_vec<T, GP, true, kTurnNone><<<n, kQkThreads, 0, s>>>(p);
+    else if (p.interleaved && p.norm)
+        k_qk_vec<T, GP, true, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
+    else if (p.interleaved)
+        k_qk_vec<T, GP, false, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
     else if (p.norm)
-        k_qk_vec<T, GP, true, false><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, GP, true, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
     else
-        k_qk_vec<T, GP, false, true><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, GP, false, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
     return cudaGetLastError();
 }
 
