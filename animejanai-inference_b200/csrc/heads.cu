@@ -33,7 +33,7 @@ struct ajib_rotary {
 namespace ajib {
 namespace {
 
-constexpr int kQkThreads = 256;
+constexpr int kQkThreads = 128;
 
 struct QkTensor {
     const void *src;
@@ -217,10 +217,12 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const F2 (&x)[4])
 // two, d / 16 of them at work) a head. HALF: chunk g of the turned components' first half and of their
 // second, so that pairs meet in a lane; otherwise chunk g of a half of what there is. A lane computes
 // its 8 angles once and walks the heads of its token, `split` groups to a token so that small batches
-// fill the machine too. U heads are in flight at a time: DRAM latency times bandwidth is some 45 KB an
-// SM, four blocks of 256 lanes with 64 bytes each hold 64 KB.
+// fill the machine too. With a norm a head is in flight at a time (64 registers, 8 blocks an SM: the
+// sum's and the square root's latency is hidden by other warps), without one two (80 registers, 6 blocks).
+// Measured, one / two heads: norms of 2040 windows 149 / 158 us, norms and rotation of 8192 tokens 46 /
+// 50, rotation alone of 2 x 4999 tokens 39 / 39, of 8 frames of 8160 76 / 70.
 template <typename T, int GP, bool NORM, int TURN>
-__global__ void __launch_bounds__(kQkThreads, TURN ? 3 : 4) k_qk_vec(const __grid_constant__ QkDev p)
+__global__ void __launch_bounds__(kQkThreads, NORM ? 8 : 6) k_qk_vec(const __grid_constant__ QkDev p)
 {
     const uint32_t slot = blockIdx.x * (kQkThreads / GP) + threadIdx.x / GP;  // (below 2^32: run_qk)
     const int g = threadIdx.x % GP;
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kQkThreads, TURN ? 3 : 4) k_qk_vec(const __gri
         const T *src = (const T *)q.src + b * q.sb + t * q.st + h * q.sh;
         T *dst = (T *)q.dst + b * q.ob + t * q.ot + h * q.oh;
         const int64_t step = p.split * q.sh, out_step = p.split * q.oh;
-        constexpr int U = 2;  // heads in flight
+        constexpr int U = NORM ? 1 : 2;  // heads in flight
         for (; h < q.heads; h += U * p.split) {  // (uniform over the lanes of a head)
             uint4 x[U][2];
 #pragma unroll
@@ -375,9 +377,17 @@ cudaError_t run_qk(QkDev &p, int width, int64_t rows, cudaStream_t s)
     const int heads = p.t[0].heads + p.t[1].heads;
     if (width == 16 && p.d % 16 == 0 && p.rot % 16 == 0 && (p.norm || p.rot)) {
         const int g = p.d / 16;
-        // groups of lanes to a token: one does all its heads once that gives every SM 2048 lanes
+        // groups of lanes to a token: one does all its heads once that gives every SM 2048 lanes; a divisor
+        // of both head counts, so that no group idles, if one is near (40 heads of 8192 tokens: 4 groups
+        // 45.6 us, 5 53.5)
         const int64_t lanes = rows * g, want = 148 * 2048;
         p.split = (int)std::min<int64_t>(heads, std::max<int64_t>(1, (want + lanes - 1) / lanes));
+        if (p.split < heads)
+            for (int s = p.split; 2 * s >= p.split; s--)
+                if (p.t[0].heads % s == 0 && p.t[1].heads % s == 0) {
+                    p.split = s;
+                    break;
+                }
         p.slots = rows * p.split;
         if (p.slots < 1ll << 31)
             return g == 1 ? run_vec<T, 1>(p, s) : g == 2 ? run_vec<T, 2>(p, s) : g <= 4 ? run_vec<T, 4>(p, s)
