@@ -1,27 +1,34 @@
 /*
- * attention_tc.cuh — attention of long prompts on the fifth-generation tensor cores (tcgen05).
+ * attention_tc.cuh — attention of prompts and windows on the fifth-generation tensor cores (tcgen05).
  *
- * A block takes 256 queries of one head as two tiles of 128 and walks the keys in tiles of 128.
- * Warps 0-3 and 4-7 do the softmax of one query tile each (a thread a row), warp 8 issues the TMA
- * copies, warps 9 and 10 the products of a query tile each (one warp for both waited for one tile's
- * softmax with the other's ready), warp 11 looks up which key tiles hold which documents:
- *   S_q = Q_q K^T   (both from shared memory)       -> TMEM, 128 columns each
- *   O_q += P_q V    (P from TMEM, V from shared)    -> TMEM, DP columns each
- * At 128 components P_q takes the columns of S_q (a thread holds its whole row of scores in registers
- * before it writes probabilities back), so TMEM's 512 columns hold both tiles. The products are issued
- * P0 V, S0', P1 V, S1': while one tile's softmax runs, the other tile's products do. Up to 64
- * components P has columns of its own and S0', S1' go first: the softmax then never waits for them.
+ * A block takes 256 queries of one head as two tiles of 128 and walks the keys in tiles (128 keys with
+ * up to 128 components a head, 64 with up to 64). Warps 0-3 and 4-7 do the softmax of one query tile
+ * each, a thread a row; warp 8 issues the TMA copies; warps 9 and 10 the products of a query tile each:
+ *   S = Q K^T   (both from shared memory)     -> TMEM
+ *   O += P V    (P from TMEM, V from shared)  -> TMEM
+ * P takes the columns of S, half as many, once they are read: 128-key tiles fill TMEM's 512 columns,
+ * 64-key tiles half of it, so that two blocks share an SM. (A products warp for both query tiles waited
+ * for one tile's softmax while the other's was ready.) Warp 11 hands out the items (sequence, head, 256
+ * queries) with their reach of keys and, where there are documents, which key tiles hold one of a
+ * query tile's, two items ahead. Blocks stay and walk items, so that copies and products of the next one run
+ * while the softmax warps still write the last one out.
  *
  * The running maximum a row is scaled by only follows the true one when that has grown by more than
- * 2^8: the accumulators are rescaled rarely, and by the softmax threads themselves, at a time when
- * no product touches them. Probabilities are then up to 2^8 instead of 1, which costs neither fp16
- * nor bf16 any precision.
+ * 2^8: the outputs are rescaled rarely, by the softmax threads themselves, at a time when no product
+ * touches them. Probabilities are then up to 2^8 instead of 1, which costs neither fp16 nor bf16 any
+ * precision.
  *
- * Blocks stay and walk items of 256 queries: copies and products of the next item run while the
- * softmax warps still write the last one out.
+ * What bounds it: per 256 x 128 scores the tensor pipe needs 32 * DP cycles (8192 flop a cycle) and the
+ * exponentials 2048 (16 a cycle): even at DP 128, where 4096 x 4096 tokens of 16 heads take 120 us (1.14
+ * PFLOP/s, 69 % of the measured matrix rate) and an 8192-token causal prompt 222 us (1.25 PFLOP/s of
+ * the pairs that are seen; events, idle card). At DP 64 it is the instructions of the softmax:
+ * about ten an element with a table's bias, half of the issue slots of an SM (2040 windows of 256 tokens, 6
+ * heads of 32: 597 us; 20 % of the exponential unit, 23 % of DRAM).
  *
- * What bounds it: per 256 x 128 scores the tensor pipe needs 32 * DP cycles (8192 flop a cycle)
- * and the exponentials 2048 (16 a cycle): even at DP 128, exponentials at 64.
+ * Tried and left out: taking turns at the exponential unit, a quarter of the exponentials as a polynomial
+ * on the FMA pipe (233 against 222 us together, they pay only while products wait for one another);
+ * two passes over the scores at DP 128 (275); one block of 128-key tiles an SM at DP 64 (windows 650, prompt
+ * 243 against 220).
  */
 #pragma once
 
@@ -359,8 +366,13 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
         tma_prefetch_desc(&mq);
         tma_prefetch_desc(&mk);
         tma_prefetch_desc(&mv);
-        for (uint32_t x = bars; x < meet + 16; x += 8)
-            mbar_init(x, x >= p_half ? 4 : x >= item_empty ? 11 : x >= item_full ? 1 : x >= p_full && x < o_full ? 4 : x >= k_empty && x < v_full || x >= v_empty && x < s_full ? 2 : 1);
+        for (uint32_t x = bars; x < meet + 16; x += 8) {
+            int arrivals = 1;
+            if ((x >= k_empty && x < v_full) || (x >= v_empty && x < s_full)) arrivals = 2;        // both products warps
+            if ((x >= p_full && x < o_full) || x >= p_half) arrivals = 4;                          // a query tile's softmax
+            if (x >= item_empty && x < p_half) arrivals = 11;                                      // all but warp 11
+            mbar_init(x, arrivals);
+        }
         fence_mbar_init();
     }
     tc_fence_before();
@@ -632,96 +644,96 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                 float now = -INFINITY;
                 if (TWICE || back) {
 #pragma unroll 1
-                for (int c0 = 0; c0 < KT; c0 += CH) {
-                    float s[CH];
+                    for (int c0 = 0; c0 < KT; c0 += CH) {
+                        float s[CH];
 #pragma unroll
-                    for (int c = 0; c < CH; c += 32) tmem_ld32(s_at + c0 + c, s + c);
-                    tmem_wait_ld();
-                    if (scaled) {
-                        if (capped) {
-                            // exponentials and reciprocals of the tanh are three times the unit's work: below the cap a
-                            // polynomial does
-                            float far = 0.f;
+                        for (int c = 0; c < CH; c += 32) tmem_ld32(s_at + c0 + c, s + c);
+                        tmem_wait_ld();
+                        if (scaled) {
+                            if (capped) {
+                                // exponentials and reciprocals of the tanh are three times the unit's work: below the cap a
+                                // polynomial does
+                                float far = 0.f;
 #pragma unroll
-                            for (int c = 0; c < CH; c += 2) far = max3(far, fabsf(s[c]), fabsf(s[c + 1]));
-                            if (__all_sync(0xffffffffu, far * fabsf(p.cap_in) <= 1.f)) {
-                                const F2 in = f2(p.cap_in, p.cap_in), out = f2(p.cap_out, p.cap_out);
+                                for (int c = 0; c < CH; c += 2) far = max3(far, fabsf(s[c]), fabsf(s[c + 1]));
+                                if (__all_sync(0xffffffffu, far * fabsf(p.cap_in) <= 1.f)) {
+                                    const F2 in = f2(p.cap_in, p.cap_in), out = f2(p.cap_out, p.cap_out);
 #pragma unroll
-                                for (int c = 0; c < CH; c += 2)
-                                    f2_out(f2_mul(f2_tanh(f2_mul(f2(s[c], s[c + 1]), in)), out), s[c], s[c + 1]);
-                            } else {
+                                    for (int c = 0; c < CH; c += 2)
+                                        f2_out(f2_mul(f2_tanh(f2_mul(f2(s[c], s[c + 1]), in)), out), s[c], s[c + 1]);
+                                } else {
 #pragma unroll
-                                for (int c = 0; c < CH; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
+                                    for (int c = 0; c < CH; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
+                                }
+                            } else if (FORM != kFormGrid && !(FORM == kFormAny && grid)) {
+#pragma unroll
+                                for (int c = 0; c < CH; c++) s[c] *= p.scale;
                             }
-                        } else if (FORM != kFormGrid && !(FORM == kFormAny && grid)) {
+                            if (FORM == kFormSlope || (FORM == kFormAny && P.bias_form == kBiasSlope)) {
+                                const float d0 = (float)(r.at - j0 - c0);
 #pragma unroll
-                            for (int c = 0; c < CH; c++) s[c] *= p.scale;
-                        }
-                        if (FORM == kFormSlope || (FORM == kFormAny && P.bias_form == kBiasSlope)) {
-                            const float d0 = (float)(r.at - j0 - c0);
+                                for (int c = 0; c < CH; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
+                            } else if (FORM == kFormAny && P.bias_form == kBiasLine) {
 #pragma unroll
-                            for (int c = 0; c < CH; c++) s[c] = fmaf(-r.slope, fabsf(d0 - (float)c), s[c]);
-                        } else if (FORM == kFormAny && P.bias_form == kBiasLine) {
+                                for (int c = 0; c < CH; c++) s[c] += table_bias(p, r, 0, j0 + c0 + c);
+                            } else if (grid) {
+                                const float f = capped ? 1.f : p.scale;
+                                const F2 ff = f2(f, f);
+                                if (quads) {
 #pragma unroll
-                            for (int c = 0; c < CH; c++) s[c] += table_bias(p, r, 0, j0 + c0 + c);
-                        } else if (grid) {
-                            const float f = capped ? 1.f : p.scale;
-                            const F2 ff = f2(f, f);
-                            if (quads) {
+                                    for (int c = 0; c < CH; c += 16) {
+                                        const int4 at = *reinterpret_cast<const int4 *>(places + ((j0 + c0 + c) >> 2));
 #pragma unroll
-                                for (int c = 0; c < CH; c += 16) {
-                                    const int4 at = *reinterpret_cast<const int4 *>(places + ((j0 + c0 + c) >> 2));
+                                        for (int y = 0; y < 16; y += 2) {
+                                            const float *e = mine + (y < 4 ? at.x : y < 8 ? at.y : y < 12 ? at.z : at.w) + (y & 3);
+                                            f2_out(f2_fma(f2(s[c + y], s[c + y + 1]), ff, f2(e[0], e[1])), s[c + y], s[c + y + 1]);
+                                        }
+                                    }
+                                } else {
 #pragma unroll
-                                    for (int y = 0; y < 16; y += 2) {
-                                        const float *e = mine + (y < 4 ? at.x : y < 8 ? at.y : y < 12 ? at.z : at.w) + (y & 3);
-                                        f2_out(f2_fma(f2(s[c + y], s[c + y + 1]), ff, f2(e[0], e[1])), s[c + y], s[c + y + 1]);
+                                    for (int c = 0; c < CH; c += 4) {
+                                        const int4 at = *reinterpret_cast<const int4 *>(places + j0 + c0 + c);
+                                        s[c] = fmaf(s[c], f, mine[at.x]);
+                                        s[c + 1] = fmaf(s[c + 1], f, mine[at.y]);
+                                        s[c + 2] = fmaf(s[c + 2], f, mine[at.z]);
+                                        s[c + 3] = fmaf(s[c + 3], f, mine[at.w]);
                                     }
                                 }
-                            } else {
+                            }
+                        }
+                        if (!all) {
 #pragma unroll
-                                for (int c = 0; c < CH; c += 4) {
-                                    const int4 at = *reinterpret_cast<const int4 *>(places + j0 + c0 + c);
-                                    s[c] = fmaf(s[c], f, mine[at.x]);
-                                    s[c + 1] = fmaf(s[c + 1], f, mine[at.y]);
-                                    s[c + 2] = fmaf(s[c + 2], f, mine[at.z]);
-                                    s[c + 3] = fmaf(s[c + 3], f, mine[at.w]);
+                            for (int w = 0; w < CH; w += 32) {
+                                // a bit a key: [0, below) or [lo, hi), below end, of this query's document
+                                const int j = j0 + c0 + w, lo = max(r.lo, 0) - j, hi = min(r.hi == INT_MAX ? INT_MAX : r.hi - j, 31) + 1;
+                                uint32_t seen = ((bits_below(hi) & ~bits_below(lo)) | bits_below(r.pre - j)) & bits_below(x.kn - j);
+                                if (docs) {
+                                    // one vote for each document among the warp's queries
+                                    const int key = __ldg(docs + min(j + lane, x.kn - 1));
+                                    for (uint32_t left = 0xffffffffu; left;) {
+                                        const int id = __shfl_sync(0xffffffffu, r.doc, __ffs(left) - 1);
+                                        const bool same = r.doc == id;
+                                        const uint32_t of = __ballot_sync(0xffffffffu, key == id);
+                                        if (same) seen &= of;
+                                        left &= ~__ballot_sync(0xffffffffu, same);
+                                    }
                                 }
+#pragma unroll
+                                for (int c = 0; c < 32; c++) s[w + c] = seen >> c & 1 ? s[w + c] : -INFINITY;
+                            }
+                        }
+                        if (TWICE) now = fmaxf(now, row_max<CH>(s));
+                        if (back) {
+#pragma unroll
+                            for (int c = 0; c < CH; c += 16) {
+                                uint32_t w[16];
+#pragma unroll
+                                for (int y = 0; y < 16; y++) w[y] = __float_as_uint(s[c + y]);
+                                tmem_st16(s_at + c0 + c, w);
                             }
                         }
                     }
-                    if (!all) {
-#pragma unroll
-                        for (int w = 0; w < CH; w += 32) {
-                            // a bit a key: [0, below) or [lo, hi), below end, of this query's document
-                            const int j = j0 + c0 + w, lo = max(r.lo, 0) - j, hi = min(r.hi == INT_MAX ? INT_MAX : r.hi - j, 31) + 1;
-                            uint32_t seen = ((bits_below(hi) & ~bits_below(lo)) | bits_below(r.pre - j)) & bits_below(x.kn - j);
-                            if (docs) {
-                                // one vote for each document among the warp's queries
-                                const int key = __ldg(docs + min(j + lane, x.kn - 1));
-                                for (uint32_t left = 0xffffffffu; left;) {
-                                    const int id = __shfl_sync(0xffffffffu, r.doc, __ffs(left) - 1);
-                                    const bool same = r.doc == id;
-                                    const uint32_t of = __ballot_sync(0xffffffffu, key == id);
-                                    if (same) seen &= of;
-                                    left &= ~__ballot_sync(0xffffffffu, same);
-                                }
-                            }
-#pragma unroll
-                            for (int c = 0; c < 32; c++) s[w + c] = seen >> c & 1 ? s[w + c] : -INFINITY;
-                        }
-                    }
-                    if (TWICE) now = fmaxf(now, row_max<CH>(s));
-                    if (back) {
-#pragma unroll
-                        for (int c = 0; c < CH; c += 16) {
-                            uint32_t w[16];
-#pragma unroll
-                            for (int y = 0; y < 16; y++) w[y] = __float_as_uint(s[c + y]);
-                            tmem_st16(s_at + c0 + c, w);
-                        }
-                    }
-                }
-                if (back) tmem_wait_st();
+                    if (back) tmem_wait_st();
                 }
                 float s[W];
                 if (!TWICE) {
