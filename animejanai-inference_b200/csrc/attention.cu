@@ -287,9 +287,10 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         p.cap_in = op->scale / op->cap;
         p.cap_out = op->cap * dev::kLog2e;
     }
-    const int far = INT_MAX / 2;
-    p.left = op->left < 0 || op->left > kMaxCount * 2 ? far : op->left;
-    p.right = op->causal ? 0 : op->right < 0 || op->right > kMaxCount * 2 ? far : op->right;
+    // (a reach that passes every distance is none; sums of a place and a reach then fit an int)
+    const int far = INT_MAX / 2, most = op->lq + op->lk;
+    p.left = op->left < 0 || op->left >= most ? far : op->left;
+    p.right = op->causal ? 0 : op->right < 0 || op->right >= most ? far : op->right;
     p.align_end = op->align_end != 0;
     p.q_len = op->q_len;
     p.k_len = op->k_len;
