@@ -52,10 +52,11 @@ size_t packed_bytes(const ajib_attn *op, int dp, int tensor)
 //   128 components, 500 tokens 27 / 14 / 19, 800 39 / 27 / 21
 // so few while all its blocks run at once, then tc; 600 windows of 144 tokens of 6 heads 303 / 723 / 169.
 // Heads of a size that TMA cannot copy (d not a multiple of 8) are copied to padded rows for tc.
-// With few queries the keys are also split until there is a block an SM or a split has only kSplitTiles
-// tiles. (us, with one / two / three blocks an SM: 2 x 16384 keys of 8 heads of 128 33 / 37 / 39, 8
-// caches of 9 to 16 thousand 78 / 79 / 75; with at least 4 / 8 tiles a split: 4000 keys 14.2 / 16.4, 1500
-// keys 12.4 / 13.9.)
+// With few queries the keys are also split until there is a block an SM (three where lengths are given,
+// which makes caches uneven) or a split has only kSplitTiles tiles. (us, with one / two / three blocks an
+// SM: 2 x 16384 keys of 8 heads of 128 33 / 37 / 39; 8 caches of 9 to 16 thousand keys 78 / 79 / 75, five
+// tokens over them 102 / 97 / 89; with at least 4 / 8 tiles a split: 4000 keys 14.2 / 16.4, 1500 keys
+// 12.4 / 13.9.)
 bool choose(const ajib_attn *op, Choice &c)
 {
     const int64_t group = op->hq / op->hk, base = (int64_t)op->batch * op->hk;
@@ -79,7 +80,7 @@ bool choose(const ajib_attn *op, Choice &c)
     }
     if ((c.few || c.keys) && few_blocks) {
         const int tiles = (op->lk + kMmaKeys - 1) / kMmaKeys;
-        const int64_t want = (sm_count() + few_blocks - 1) / few_blocks;
+        const int64_t want = ((op->k_len ? 3 : 1) * (int64_t)sm_count() + few_blocks - 1) / few_blocks;
         c.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, tiles / kSplitTiles), kMaxSplits));
         if (few_blocks * c.nsplit > 0x7fffffff) return false;
         if (c.nsplit > 1) c.space = (size_t)(base * c.rows * c.nsplit) * (8 + (size_t)op->d * 4);
