@@ -306,9 +306,13 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
     p.reach_x = op->reach_x;
     p.masked = p.left != far || p.right != far || p.q_doc;
     m.rows = (int)c.rows;
-    m.wq = heads_width(q, b, op->lq, op->hq, d);
-    m.wo = heads_width(out, b, op->lq, op->hq, d);
-    m.wkv = op->lk ? std::min(heads_width(k, b, op->lk, op->hk, d), heads_width(v, b, op->lk, op->hk, d)) : 16;
+    auto copies = [&](const ajib_heads *x, int tokens, int heads) {  // of 16, 4 or 2 bytes
+        const int w = heads_width(x, b, tokens, heads, d);
+        return w == 8 ? 4 : w;
+    };
+    m.wq = copies(q, op->lq, op->hq);
+    m.wo = copies(out, op->lq, op->hq);
+    m.wkv = op->lk ? std::min(copies(k, op->lk, op->hk), copies(v, op->lk, op->hk)) : 16;
     const int64_t slots = (int64_t)b * op->hk * c.rows * c.nsplit;
     m.part_ml = (float2 *)workspace;
     m.part = (float *)workspace + 2 * slots;

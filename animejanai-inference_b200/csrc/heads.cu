@@ -47,7 +47,7 @@ struct QkDev {
     QkTensor t[2];
     const int *pos, *len;
     int64_t pos_sb, slots;
-    int pos0, tokens, d, rot, axes, grid_w, interleaved, norm, split;
+    int pos0, tokens, d, rot, axes, grid_w, interleaved, norm, split, lanes_log2;
     float eps, amplitude, inv_d, inv_eps;
     uint64_t turns[kMaxHeadDim / 2];
 };
@@ -183,13 +183,25 @@ using dev::f2_fma;
 using dev::f2_mul;
 using dev::f2_out;
 
-// The sum of the squares of a lane's 16 components times scale.
-__device__ __forceinline__ float sum_squares(const F2 (&a)[4], const F2 (&e)[4], float scale)
+// A lane's chunk of CS components, moved by one access.
+template <int CS> struct Chunk;
+template <> struct Chunk<8> {
+    using V = uint4;
+};
+template <> struct Chunk<4> {
+    using V = uint2;
+};
+template <> struct Chunk<2> {
+    using V = uint32_t;
+};
+
+// The sum of the squares of a lane's components times scale.
+template <int N> __device__ __forceinline__ float sum_squares(const F2 (&a)[N], const F2 (&e)[N], float scale)
 {
     const F2 by = f2(scale, scale);
     F2 sum = f2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < N; i++) {
         const F2 x = f2_mul(a[i], by), y = f2_mul(e[i], by);
         sum = f2_fma(x, x, f2_fma(y, y, sum));
     }
@@ -198,84 +210,101 @@ __device__ __forceinline__ float sum_squares(const F2 (&a)[4], const F2 (&e)[4],
     return lo + hi;
 }
 
-enum { kTurnNone = 0, kTurnHalf = 1, kTurnInterleaved = 2 };
-
-template <typename T> __device__ __forceinline__ uint4 pack8(const F2 (&x)[4])
+template <typename T, int CS> __device__ __forceinline__ typename Chunk<CS>::V pack_chunk(const F2 (&x)[CS / 2])
 {
-    uint32_t w[4];
+    union {
+        uint32_t w[CS / 2];
+        typename Chunk<CS>::V v;
+    } u;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < CS / 2; i++) {
         float lo, hi;
         f2_out(x[i], lo, hi);
-        w[i] = Pair<T>::pack(lo, hi);
+        u.w[i] = Pair<T>::pack(lo, hi);
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return u.v;
+}
+template <typename T, int CS> __device__ __forceinline__ void unpack_chunk(const typename Chunk<CS>::V &v, F2 (&x)[CS / 2])
+{
+    union {
+        uint32_t w[CS / 2];
+        typename Chunk<CS>::V v;
+    } u;
+    u.v = v;
+#pragma unroll
+    for (int i = 0; i < CS / 2; i++) {
+        const float2 f = Pair<T>::unpack(u.w[i]);
+        x[i] = f2(f.x, f.y);
+    }
 }
 
-// d and the turned components multiples of 16, every row 16-byte aligned: a lane holds two chunks of 8
-// components of a head (16-byte loads, neighbouring lanes on neighbouring chunks), GP lanes (a power of
-// two, d / 16 of them at work) a head. HALF: chunk g of the turned components' first half and of their
-// second, so that pairs meet in a lane; otherwise chunk g of a half of what there is. A lane computes
-// its 8 angles once and walks the heads of its token, `split` groups to a token so that small batches
-// fill the machine too. With a norm a head is in flight at a time (64 registers, 8 blocks an SM: the
-// sum's and the square root's latency is hidden by other warps), without one two (80 registers, 6 blocks).
-// Measured, one / two heads: norms of 2040 windows 149 / 158 us, norms and rotation of 8192 tokens 46 /
-// 50, rotation alone of 2 x 4999 tokens 39 / 39, of 8 frames of 8160 76 / 70.
-template <typename T, int GP, bool NORM, int TURN>
+enum { kTurnNone = 0, kTurnHalf = 1, kTurnInterleaved = 2 };
+
+// A lane holds two chunks of CS components of a head (accesses of 2 CS bytes, neighbouring lanes on
+// neighbouring chunks), a power of two of lanes a head. HALF: chunk g of the turned components' first half
+// and of their second, so that pairs meet in a lane; otherwise chunk g of a half of what there is, or two
+// in a row where that does not divide. A lane computes its CS angles once and walks the heads of its token,
+// `split` groups to a token so that small batches fill the machine too. With a norm a head is in
+// flight at a time (64 registers, 8 blocks an SM: the sum's and the square root's latency is hidden by other
+// warps), without one two (80 registers, 6 blocks). Measured, one / two heads: norms of 2040 windows 149 /
+// 158 us, norms and rotation of 8192 tokens 46 / 50, rotation alone of 2 x 4999 tokens 39 / 39, of 8 frames
+// of 8160 76 / 70.
+template <typename T, int CS, bool NORM, int TURN>
 __global__ void __launch_bounds__(kQkThreads, NORM ? 8 : 6) k_qk_vec(const __grid_constant__ QkDev p)
 {
-    const uint32_t slot = blockIdx.x * (kQkThreads / GP) + threadIdx.x / GP;  // (below 2^32: run_qk)
-    const int g = threadIdx.x % GP;
+    using V = typename Chunk<CS>::V;
+    constexpr int N = CS / 2;
+    const uint32_t slot = (blockIdx.x * kQkThreads + threadIdx.x) >> p.lanes_log2;  // (lanes below 2^32: run_qk)
+    const int lanes = 1 << p.lanes_log2, g = threadIdx.x & (lanes - 1);
     const bool there = slot < (uint32_t)p.slots;
     const uint32_t at = there ? slot : (uint32_t)p.slots - 1;
     const uint32_t bt = at / p.split;
     const int h0 = (int)(at - bt * p.split);
     const int b = (int)(bt / p.tokens), t = (int)(bt - (uint32_t)b * p.tokens);
-    // lanes of a warp stay together for the sums: what a lane has no part in, it neither reads nor writes
-    const bool live = there && g * 16 < p.d && !(p.len && t >= p.len[b]);
     constexpr bool apart = TURN == kTurnHalf;
-    int c1 = 8 * g, c2 = (p.d >> 1) + 8 * g;
-    if (apart) {
-        const int turned = p.rot >> 4, rest = (p.d - p.rot) >> 1;  // lanes at work on each part
-        c1 = g < turned ? 8 * g : p.rot + 8 * (g - turned);
-        c2 = c1 + (g < turned ? p.rot >> 1 : rest);
-    }
+    // the part of the head that this lane has chunks of: what turns (HALF), the rest, or all
+    const int turned = apart ? p.rot / (2 * CS) : 0;
+    const bool in_turned = g < turned;
+    const int from = apart && !in_turned ? p.rot : 0, size = in_turned ? p.rot : p.d - from, k = g - (in_turned ? 0 : turned);
+    const bool halves = size % (2 * CS) == 0;
+    const int c1 = from + (halves ? CS * k : 2 * CS * k), c2 = c1 + (halves ? size >> 1 : CS);
+    // lanes of a warp stay together for the sums: what a lane has no part in, it neither reads nor writes
+    const bool here = there && !(p.len && t >= p.len[b]);
+    const bool live1 = here && c1 < p.d && (!halves || CS * k < size >> 1), live2 = live1 && c2 < p.d;
     // HALF: c, s, sn = cos, sin, -sin of the chunk's pairs; INTERLEAVED: c, sn = (cos, cos), (-sin, sin) of
     // the first chunk's pairs and s, ce the same of the second's
-    F2 c[4], s[4], sn[4], ce[4];
+    F2 c[N], s[N], sn[N], ce[N];
     if (TURN) {
-        float co[8], si[8];
+        float co[CS], si[CS];
 #pragma unroll
-        for (int i = 0; i < 8; i++) co[i] = 1.f, si[i] = 0.f;
-        if (live && c1 < p.rot) {
+        for (int i = 0; i < CS; i++) co[i] = 1.f, si[i] = 0.f;
+        if (live1 && c1 < p.rot) {
             const Place place = place_of(p, position_of(p, b, t));
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int pair = apart ? c1 + i : (i < 4 ? c1 >> 1 : (c2 >> 1) - 4) + i;
+            for (int i = 0; i < CS; i++) {
+                const int pair = apart ? c1 + i : (i < N ? c1 >> 1 : (c2 >> 1) - N) + i;
                 if (2 * pair < p.rot) pair_angle(p, place, pair, co[i], si[i]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < N; i++) {
             c[i] = apart ? f2(co[2 * i], co[2 * i + 1]) : f2(co[i], co[i]);
-            s[i] = apart ? f2(si[2 * i], si[2 * i + 1]) : f2(co[4 + i], co[4 + i]);
+            s[i] = apart ? f2(si[2 * i], si[2 * i + 1]) : f2(co[N + i], co[N + i]);
             sn[i] = apart ? f2(-si[2 * i], -si[2 * i + 1]) : f2(-si[i], si[i]);
-            ce[i] = f2(-si[4 + i], si[4 + i]);
+            ce[i] = f2(-si[N + i], si[N + i]);
         }
     }
-    const unsigned all = ((1u << GP) - 1) << (threadIdx.x % 32 / GP * GP);
+    const unsigned all = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << ((threadIdx.x & 31) & ~(lanes - 1));
     int h = h0;
     for (int part = 0; part < 2; part++) {
         const QkTensor &q = p.t[part];
-        F2 w1[4], w2[4];
+        F2 w1[N], w2[N];
         if (NORM) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < N; i++) {
                 w1[i] = w2[i] = f2(1.f, 1.f);
-                if (live && q.w) {
-                    w1[i] = f2(__ldg(q.w + c1 + 2 * i), __ldg(q.w + c1 + 2 * i + 1));
-                    w2[i] = f2(__ldg(q.w + c2 + 2 * i), __ldg(q.w + c2 + 2 * i + 1));
-                }
+                if (live1 && q.w) w1[i] = f2(__ldg(q.w + c1 + 2 * i), __ldg(q.w + c1 + 2 * i + 1));
+                if (live2 && q.w) w2[i] = f2(__ldg(q.w + c2 + 2 * i), __ldg(q.w + c2 + 2 * i + 1));
             }
         }
         const T *src = (const T *)q.src + b * q.sb + t * q.st + h * q.sh;
@@ -283,65 +312,60 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? 8 : 6) k_qk_vec(const __gri
         const int64_t step = p.split * q.sh, out_step = p.split * q.oh;
         constexpr int U = NORM ? 1 : 2;  // heads in flight
         for (; h < q.heads; h += U * p.split) {  // (uniform over the lanes of a head)
-            uint4 x[U][2];
+            V x[U][2];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
-                if (live && h + u * p.split < q.heads) {
-                    x[u][0] = *reinterpret_cast<const uint4 *>(src + u * step + c1);
-                    x[u][1] = *reinterpret_cast<const uint4 *>(src + u * step + c2);
+                x[u][0] = x[u][1] = V{};
+                if (h + u * p.split < q.heads) {
+                    if (live1) x[u][0] = *reinterpret_cast<const V *>(src + u * step + c1);
+                    if (live2) x[u][1] = *reinterpret_cast<const V *>(src + u * step + c2);
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                F2 a[4], e[4];
-                const uint32_t *xa = &x[u][0].x, *xe = &x[u][1].x;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 fa = Pair<T>::unpack(xa[i]), fe = Pair<T>::unpack(xe[i]);
-                    a[i] = f2(fa.x, fa.y);
-                    e[i] = f2(fe.x, fe.y);
-                }
+                F2 a[N], e[N];
+                unpack_chunk<T, CS>(x[u][0], a);
+                unpack_chunk<T, CS>(x[u][1], e);
                 if (NORM) {
-                    float sum = sum_squares(a, e, 1.f);
-#pragma unroll
-                    for (int m = GP / 2; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
+                    float sum = sum_squares<N>(a, e, 1.f);
+                    for (int m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
                     const float scale = rescale_of(p, sum);
                     if (scale != 1.f) {  // (every lane of the head agrees)
-                        sum = sum_squares(a, e, scale);
-                        for (int m = GP / 2; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
+                        sum = sum_squares<N>(a, e, scale);
+                        for (int m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
                     }
                     const float f = norm_factor(p, sum, scale);
                     const F2 ff = f2(f, f);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < N; i++) {
                         a[i] = f2_mul(f2_mul(a[i], ff), w1[i]);
                         e[i] = f2_mul(f2_mul(e[i], ff), w2[i]);
                     }
                 }
-                if (TURN) {  // (what does not turn has angle 0)
-                    if (apart) {
+                // (what does not turn has angle 0; an infinity or a NaN there meets no partner)
+                if (apart) {
+                    if (in_turned) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < N; i++) {
                             const F2 x1 = a[i], x2 = e[i];
                             a[i] = f2_fma(x1, c[i], f2_mul(x2, sn[i]));
                             e[i] = f2_fma(x2, c[i], f2_mul(x1, s[i]));
                         }
-                    } else {
-                        // a chunk is x1, x2 pairs: c holds an angle twice, sn its sine as -s, s
+                    }
+                } else if (TURN) {
+                    // a chunk is x1, x2 pairs
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            float x1, x2, y1, y2;
-                            f2_out(a[i], x1, x2);
-                            f2_out(e[i], y1, y2);
-                            a[i] = f2_fma(a[i], c[i], f2_mul(f2(x2, x1), sn[i]));
-                            e[i] = f2_fma(e[i], s[i], f2_mul(f2(y2, y1), ce[i]));
-                        }
+                    for (int i = 0; i < N; i++) {
+                        float x1, x2, y1, y2;
+                        f2_out(a[i], x1, x2);
+                        f2_out(e[i], y1, y2);
+                        if (c1 < p.rot) a[i] = f2_fma(a[i], c[i], f2_mul(f2(x2, x1), sn[i]));
+                        if (c2 < p.rot) e[i] = f2_fma(e[i], s[i], f2_mul(f2(y2, y1), ce[i]));
                     }
                 }
-                if (live && h + u * p.split < q.heads) {
-                    *reinterpret_cast<uint4 *>(dst + u * out_step + c1) = pack8<T>(a);
-                    *reinterpret_cast<uint4 *>(dst + u * out_step + c2) = pack8<T>(e);
+                if (h + u * p.split < q.heads) {
+                    if (live1) *reinterpret_cast<V *>(dst + u * out_step + c1) = pack_chunk<T, CS>(a);
+                    if (live2) *reinterpret_cast<V *>(dst + u * out_step + c2) = pack_chunk<T, CS>(e);
                 }
             }
             src += U * step;
@@ -352,31 +376,40 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? 8 : 6) k_qk_vec(const __gri
     }
 }
 
-template <typename T, int GP>
+template <typename T, int CS>
 cudaError_t run_vec(const QkDev &p, cudaStream_t s)
 {
-    const int64_t blocks = (p.slots * GP + kQkThreads - 1) / kQkThreads;
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    const unsigned n = (unsigned)blocks;
+    const unsigned n = (unsigned)(((p.slots << p.lanes_log2) + kQkThreads - 1) / kQkThreads);
     if (!p.rot)
-        k_qk_vec<T, GP, true, kTurnNone><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, true, kTurnNone><<<n, kQkThreads, 0, s>>>(p);
     else if (p.interleaved && p.norm)
-        k_qk_vec<T, GP, true, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, true, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
     else if (p.interleaved)
-        k_qk_vec<T, GP, false, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, false, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
     else if (p.norm)
-        k_qk_vec<T, GP, true, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, true, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
     else
-        k_qk_vec<T, GP, false, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, false, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
     return cudaGetLastError();
+}
+
+// How many lanes of two chunks of cs components a head takes, 0 where it does not divide into them.
+int lanes_of(const QkDev &p, int cs, int width)
+{
+    if (width < 2 * cs || p.d % cs || p.rot % (p.interleaved ? cs : 2 * cs)) return 0;
+    const int turned = p.interleaved ? 0 : p.rot, lanes = turned / (2 * cs) + (p.d - turned + 2 * cs - 1) / (2 * cs);
+    return lanes <= 32 ? lanes : 0;
 }
 
 template <typename T>
 cudaError_t run_qk(QkDev &p, int width, int64_t rows, cudaStream_t s)
 {
     const int heads = p.t[0].heads + p.t[1].heads;
-    if (width == 16 && p.d % 16 == 0 && p.rot % 16 == 0 && (p.norm || p.rot)) {
-        const int g = p.d / 16;
+    for (int cs = p.norm || p.rot ? 8 : 0; cs >= 2; cs >>= 1) {
+        const int g = lanes_of(p, cs, width);
+        if (!g) continue;
+        p.lanes_log2 = 0;
+        while (1 << p.lanes_log2 < g) p.lanes_log2++;
         // groups of lanes to a token: one does all its heads once that gives every SM 2048 lanes; a divisor
         // of both head counts, so that no group idles, if one is near (40 heads of 8192 tokens: 4 groups
         // 45.6 us, 5 53.5)
@@ -389,9 +422,8 @@ cudaError_t run_qk(QkDev &p, int width, int64_t rows, cudaStream_t s)
                     break;
                 }
         p.slots = rows * p.split;
-        if (p.slots < 1ll << 31)
-            return g == 1 ? run_vec<T, 1>(p, s) : g == 2 ? run_vec<T, 2>(p, s) : g <= 4 ? run_vec<T, 4>(p, s)
-                   : g <= 8 ? run_vec<T, 8>(p, s) : run_vec<T, 16>(p, s);
+        if (p.slots << p.lanes_log2 < 1ll << 31)
+            return cs == 8 ? run_vec<T, 8>(p, s) : cs == 4 ? run_vec<T, 4>(p, s) : run_vec<T, 2>(p, s);
     }
     p.slots = rows * heads;
     const int64_t blocks = (p.slots * 32 + kQkThreads - 1) / kQkThreads;

@@ -51,7 +51,7 @@ inline bool heads_same(const ajib_heads *a, const ajib_heads *b)
     return a->p == b->p && a->sb == b->sb && a->st == b->st && a->sh == b->sh;
 }
 
-// The widest copy, in bytes, that every row of components allows: 16, 4 or 2. (A stride of a
+// The widest copy, in bytes, that every row of components allows: 16, 8, 4 or 2. (A stride of a
 // dimension of one element is never used.)
 inline int heads_width(const ajib_heads *x, int batch, int tokens, int heads, int d)
 {
@@ -59,7 +59,7 @@ inline int heads_width(const ajib_heads *x, int batch, int tokens, int heads, in
     if (batch > 1) bits |= (uint64_t)x->sb * 2;
     if (tokens > 1) bits |= (uint64_t)x->st * 2;
     if (heads > 1) bits |= (uint64_t)x->sh * 2;
-    return (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 2;
+    return (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : 2;
 }
 
 }  // namespace ajib
