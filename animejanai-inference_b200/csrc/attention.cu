@@ -23,7 +23,7 @@ namespace {
 using namespace dev;
 
 constexpr int kSplitTiles = 4;   // at least this many key tiles a split
-constexpr int kTcQueries = 96;  // tcgen05 from here on (queries and keys)
+constexpr int kTcQueries = 32;  // tcgen05 from here on (queries and keys)
 
 // How an op runs, from its sizes alone (the workspace must be known before the launch).
 struct Choice {
@@ -50,7 +50,8 @@ size_t packed_bytes(const ajib_attn *op, int dp, int tensor)
 // Which kernel. Measured (us, 8 heads, causal; k_attn_mma / few / tc):
 //   64 components, 200 tokens 12.3 / 9.0 / 14.4, 800 26 / 18 / 27; 16 sequences of 150 20 / 23 / 14
 //   128 components, 500 tokens 27 / 14 / 19, 800 39 / 27 / 21
-// so few while all its blocks run at once, then tc; 600 windows of 144 tokens of 6 heads 303 / 723 / 169.
+// so few while all its blocks run at once, then tc: 600 windows of 144 tokens of 6 heads 303 / 723 / 169, 464
+// windows of 64 of 3 heads - / 97 / 27 (below kTcQueries few again, whose blocks hold 16 rows).
 // Heads of a size that TMA cannot copy (d not a multiple of 8) are copied to padded rows for tc.
 // With few queries the keys are also split until there is a block an SM (three where lengths are given,
 // which makes caches uneven) or a split has only kSplitTiles tiles. (us, with one / two / three blocks an
@@ -68,8 +69,9 @@ bool choose(const ajib_attn *op, Choice &c)
     if (base * c.row_tiles > 0x7fffffff) return false;
     c.keys = c.rows <= 64;
     const int fit = sm_count() * (op->d <= 64 ? FewCfg<64>::BLOCKS : op->d <= 128 ? FewCfg<128>::BLOCKS : FewCfg<256>::BLOCKS);
-    c.few = op->lk && !op->q_doc && op->d % 8 == 0 && few_blocks <= 0x7fffffff && (c.keys || few_blocks <= fit);
-    if (!c.few && !c.keys && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d <= 128) {
+    const bool tma = op->lk && !op->q_doc && op->d % 8 == 0 && few_blocks <= 0x7fffffff;
+    c.few = tma && few_blocks <= fit;
+    if (!c.few && op->lq >= kTcQueries && op->lk >= kTcQueries && op->d <= 128) {
         const bool grid = op->bias == AJIB_BIAS_TABLE && op->grid_w;
         c.tc = (!grid || grid_reached(op)) && (int64_t)op->batch * op->hq * ((op->lq + 255) / 256) <= 0x7fffffff &&
                (op->d <= 64 ? TcCfg<64>::smem(op) : TcCfg<128>::smem(op)) <= kMaxSmem;
@@ -78,7 +80,8 @@ bool choose(const ajib_attn *op, Choice &c)
             for (int i = 0; i < 3; i++) c.space += packed_bytes(op, c.pack, i);
         }
     }
-    if ((c.few || c.keys) && few_blocks) {
+    if (!c.tc && c.keys) c.few = tma;  // few queries of many sequences
+    if (!c.tc && (c.few || c.keys) && few_blocks) {
         const int tiles = (op->lk + kMmaKeys - 1) / kMmaKeys;
         const int64_t want = ((op->k_len ? 3 : 1) * (int64_t)sm_count() + few_blocks - 1) / few_blocks;
         c.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, tiles / kSplitTiles), kMaxSplits));

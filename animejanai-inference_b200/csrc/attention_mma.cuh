@@ -165,6 +165,26 @@ __device__ __forceinline__ void load_tile(uint32_t dst, char *dst_generic, int d
     }
 }
 
+// The smallest and largest of a key tile's n documents, with as many loads in flight as fit.
+template <int KT> __device__ __forceinline__ void document_range(const int *ids, int n, int &lo, int &hi)
+{
+    if (((uintptr_t)ids & 15) == 0 && n == KT) {
+#pragma unroll 8
+        for (int v = 0; v < KT; v += 4) {
+            const int4 id = __ldg(reinterpret_cast<const int4 *>(ids + v));
+            lo = min(min(lo, min(id.x, id.y)), min(id.z, id.w));
+            hi = max(max(hi, max(id.x, id.y)), max(id.z, id.w));
+        }
+    } else {
+#pragma unroll 8
+        for (int v = 0; v < n; v++) {
+            const int id = __ldg(ids + v);
+            lo = min(lo, id);
+            hi = max(hi, id);
+        }
+    }
+}
+
 // Keys [lo, hi) that some query standing from `first` to `last` sees.
 __device__ __forceinline__ void reach_of(const AttnDev &p, int first, int last, int pre, int kn, int &lo, int &hi)
 {
@@ -331,12 +351,7 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
             // lane l looks at tile w * 32 + l, so that its loads are in flight together
             const int t = w * 32 + lane;
             int klo = INT_MAX, khi = INT_MIN;
-            if (t >= t0 && t < t1)
-                for (int j = t * kMmaKeys; j < min((t + 1) * kMmaKeys, kn); j++) {
-                    const int x = __ldg(docs + j);
-                    klo = min(klo, x);
-                    khi = max(khi, x);
-                }
+            if (t >= t0 && t < t1) document_range<kMmaKeys>(docs + t * kMmaKeys, min(kn - t * kMmaKeys, kMmaKeys), klo, khi);
             const uint32_t seen = __ballot_sync(0xffffffffu, khi >= 0 && max(lo, 0) <= khi && klo <= hi);
             const uint32_t whole = __ballot_sync(0xffffffffu, lo >= 0 && lo == hi && klo == lo && khi == lo);
             if (lane == 0) {

@@ -295,28 +295,11 @@ template <int KT> __device__ __forceinline__ void document_tiles(const AttnDev &
         lo[q] = __reduce_min_sync(0xffffffffu, lo[q]);
         hi[q] = __reduce_max_sync(0xffffffffu, hi[q]);
     }
-    const bool wide = ((uintptr_t)kd & 15) == 0;
     int t_first = x.t1, t_last = x.t0 - 1;
     for (int w = x.word0; w * 32 < x.t1; w++) {
         const int t = w * 32 + lane, j = t * KT, n = min(x.kn - j, KT);
         int klo = INT_MAX, khi = INT_MIN;
-        if (t >= x.t0 && t < x.t1) {
-            if (wide && n == KT) {
-#pragma unroll 8
-                for (int v = 0; v < KT; v += 4) {
-                    const int4 id = __ldg(reinterpret_cast<const int4 *>(kd + j + v));
-                    klo = min(min(klo, min(id.x, id.y)), min(id.z, id.w));
-                    khi = max(max(khi, max(id.x, id.y)), max(id.z, id.w));
-                }
-            } else {
-#pragma unroll 8
-                for (int v = 0; v < n; v++) {
-                    const int id = __ldg(kd + j + v);
-                    klo = min(klo, id);
-                    khi = max(khi, id);
-                }
-            }
-        }
+        if (t >= x.t0 && t < x.t1) document_range<KT>(kd + j, n, klo, khi);
         uint32_t either = 0;
 #pragma unroll
         for (int q = 0; q < 2; q++) {

@@ -245,12 +245,12 @@ enum { kTurnNone = 0, kTurnHalf = 1, kTurnInterleaved = 2 };
 // and of their second, so that pairs meet in a lane; otherwise chunk g of a half of what there is, or two
 // in a row where that does not divide. A lane computes its CS angles once and walks the heads of its token,
 // `split` groups to a token so that small batches fill the machine too. With a norm a head is in
-// flight at a time (64 registers, 8 blocks an SM: the sum's and the square root's latency is hidden by other
+// flight at a time (64 to 72 registers, 7 or 8 blocks an SM: the sum's and the square root's latency is hidden by other
 // warps), without one two (80 registers, 6 blocks). Measured, one / two heads: norms of 2040 windows 149 /
 // 158 us, norms and rotation of 8192 tokens 46 / 50, rotation alone of 2 x 4999 tokens 39 / 39, of 8 frames
 // of 8160 76 / 70.
 template <typename T, int CS, bool NORM, int TURN>
-__global__ void __launch_bounds__(kQkThreads, NORM ? 8 : 6) k_qk_vec(const __grid_constant__ QkDev p)
+__global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_vec(const __grid_constant__ QkDev p)
 {
     using V = typename Chunk<CS>::V;
     constexpr int N = CS / 2;
