@@ -179,3 +179,37 @@ def test_other_stream_and_graph():
     g.replay()
     torch.cuda.synchronize()
     assert not torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d,rot", [(24, 12), (24, 24), (80, 40), (20, 20), (12, 8), (28, 4), (130, 4), (250, 250), (250, 64), (6, 4),
+                                   (2, 2), (4, 4), (26, 24), (52, 16), (104, 72), (40, 24)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("norm", [None, "rms", "l2"])
+def test_chunk_sizes(d, rot, layout, norm):
+    """Head sizes and turned parts that chunks of 8, 4 or 2 components divide, or none does."""
+    run(d=d, rot=rot, layout=layout, norm=norm, tokens=9, hq=5, hk=3)
+    run(d=d, rot=rot, layout=layout, norm=norm, tokens=300, batch=1, hq=4, hk=2, inplace=True, dtype="bf16")
+    run(d=d, rot=rot, layout=layout, norm=norm, tokens=40, hq=2, hk=0, lens=[17, 40])
+    if norm:
+        run(d=d, rot=0, norm=norm, tokens=33)
+
+
+@pytest.mark.parametrize("d,rot", [(64, 32), (30, 16), (24, 8)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_infinities_stay_in_their_pair(d, rot, layout):
+    import ajib
+    x = torch.randn(1, 3, 2, d, device="cuda").half()
+    x[0, 1, 0, rot + 1] = math.inf
+    x[0, 2, 1, 0] = math.nan
+    out = torch.empty_like(x)
+    r = ajib.Rotary(rot, layout=ajib.ROTARY_HALF if layout == "half" else ajib.ROTARY_INTERLEAVED)
+    op = ajib.qk_op(ajib.F16, 1, 3, 2, 0, d, rotary=r, pos0=5)
+    assert ajib.qk(op, H(ajib, x), None, H(ajib, out), None, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out[0, 1, 0, rot:], x[0, 1, 0, rot:])
+    bad = torch.isnan(out[0, 2, 1]).nonzero().flatten().tolist()
+    assert bad == ([0, rot // 2] if layout == "half" else [0, 1])
+    rest = out.clone()
+    rest[0, 2, 1, bad] = 0
+    rest[0, 1, 0, rot + 1] = 0
+    assert torch.isfinite(rest).all()
