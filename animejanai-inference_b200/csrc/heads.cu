@@ -249,7 +249,9 @@ enum { kTurnNone = 0, kTurnHalf = 1, kTurnInterleaved = 2 };
 // warps), without one two (80 registers, 6 blocks). Measured, one / two heads: norms of 2040 windows 149 /
 // 158 us, norms and rotation of 8192 tokens 46 / 50, rotation alone of 2 x 4999 tokens 39 / 39, of 8 frames
 // of 8160 76 / 70.
-template <typename T, int CS, bool NORM, int TURN>
+// WHOLE: every component turns, or none, and the head divides into pairs of chunks, which spares the
+// lanes the question (norms and rotation of 8192 tokens 30 M instructions, 49 us, without it).
+template <typename T, int CS, bool NORM, int TURN, bool WHOLE>
 __global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_vec(const __grid_constant__ QkDev p)
 {
     using V = typename Chunk<CS>::V;
@@ -263,14 +265,14 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_ve
     const int b = (int)(bt / p.tokens), t = (int)(bt - (uint32_t)b * p.tokens);
     constexpr bool apart = TURN == kTurnHalf;
     // the part of the head that this lane has chunks of: what turns (HALF), the rest, or all
-    const int turned = apart ? p.rot / (2 * CS) : 0;
-    const bool in_turned = g < turned;
-    const int from = apart && !in_turned ? p.rot : 0, size = in_turned ? p.rot : p.d - from, k = g - (in_turned ? 0 : turned);
-    const bool halves = size % (2 * CS) == 0;
+    const int turned = apart && !WHOLE ? p.rot / (2 * CS) : 0;
+    const bool in_turned = WHOLE || g < turned;
+    const int from = apart && !in_turned ? p.rot : 0, size = WHOLE ? p.d : in_turned ? p.rot : p.d - from, k = g - (in_turned ? 0 : turned);
+    const bool halves = WHOLE || size % (2 * CS) == 0;
     const int c1 = from + (halves ? CS * k : 2 * CS * k), c2 = c1 + (halves ? size >> 1 : CS);
     // lanes of a warp stay together for the sums: what a lane has no part in, it neither reads nor writes
     const bool here = there && !(p.len && t >= p.len[b]);
-    const bool live1 = here && c1 < p.d && (!halves || CS * k < size >> 1), live2 = live1 && c2 < p.d;
+    const bool live1 = here && c1 < p.d && (!halves || CS * k < size >> 1), live2 = live1 && (WHOLE || c2 < p.d);
     // HALF: c, s, sn = cos, sin, -sin of the chunk's pairs; INTERLEAVED: c, sn = (cos, cos), (-sin, sin) of
     // the first chunk's pairs and s, ce the same of the second's
     F2 c[N], s[N], sn[N], ce[N];
@@ -278,12 +280,12 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_ve
         float co[CS], si[CS];
 #pragma unroll
         for (int i = 0; i < CS; i++) co[i] = 1.f, si[i] = 0.f;
-        if (live1 && c1 < p.rot) {
+        if (live1 && (WHOLE || c1 < p.rot)) {
             const Place place = place_of(p, position_of(p, b, t));
 #pragma unroll
             for (int i = 0; i < CS; i++) {
                 const int pair = apart ? c1 + i : (i < N ? c1 >> 1 : (c2 >> 1) - N) + i;
-                if (2 * pair < p.rot) pair_angle(p, place, pair, co[i], si[i]);
+                if (WHOLE || 2 * pair < p.rot) pair_angle(p, place, pair, co[i], si[i]);
             }
         }
 #pragma unroll
@@ -359,8 +361,8 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_ve
                         float x1, x2, y1, y2;
                         f2_out(a[i], x1, x2);
                         f2_out(e[i], y1, y2);
-                        if (c1 < p.rot) a[i] = f2_fma(a[i], c[i], f2_mul(f2(x2, x1), sn[i]));
-                        if (c2 < p.rot) e[i] = f2_fma(e[i], s[i], f2_mul(f2(y2, y1), ce[i]));
+                        if (WHOLE || c1 < p.rot) a[i] = f2_fma(a[i], c[i], f2_mul(f2(x2, x1), sn[i]));
+                        if (WHOLE || c2 < p.rot) e[i] = f2_fma(e[i], s[i], f2_mul(f2(y2, y1), ce[i]));
                     }
                 }
                 if (h + u * p.split < q.heads) {
@@ -376,21 +378,28 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_ve
     }
 }
 
-template <typename T, int CS>
-cudaError_t run_vec(const QkDev &p, cudaStream_t s)
+template <typename T, int CS, bool WHOLE>
+cudaError_t run_vec_form(const QkDev &p, cudaStream_t s)
 {
     const unsigned n = (unsigned)(((p.slots << p.lanes_log2) + kQkThreads - 1) / kQkThreads);
     if (!p.rot)
-        k_qk_vec<T, CS, true, kTurnNone><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, true, kTurnNone, WHOLE><<<n, kQkThreads, 0, s>>>(p);
     else if (p.interleaved && p.norm)
-        k_qk_vec<T, CS, true, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, true, kTurnInterleaved, WHOLE><<<n, kQkThreads, 0, s>>>(p);
     else if (p.interleaved)
-        k_qk_vec<T, CS, false, kTurnInterleaved><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, false, kTurnInterleaved, WHOLE><<<n, kQkThreads, 0, s>>>(p);
     else if (p.norm)
-        k_qk_vec<T, CS, true, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, true, kTurnHalf, WHOLE><<<n, kQkThreads, 0, s>>>(p);
     else
-        k_qk_vec<T, CS, false, kTurnHalf><<<n, kQkThreads, 0, s>>>(p);
+        k_qk_vec<T, CS, false, kTurnHalf, WHOLE><<<n, kQkThreads, 0, s>>>(p);
     return cudaGetLastError();
+}
+
+template <typename T, int CS>
+cudaError_t run_vec(const QkDev &p, cudaStream_t s)
+{
+    const bool whole = (!p.rot || p.rot == p.d) && p.d % (2 * CS) == 0;
+    return whole ? run_vec_form<T, CS, true>(p, s) : run_vec_form<T, CS, false>(p, s);
 }
 
 // How many lanes of two chunks of cs components a head takes, 0 where it does not divide into them.
