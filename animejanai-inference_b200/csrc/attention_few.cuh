@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<DP>::BLOCKS)
     const int pre = p.prefix ? max(__ldg(p.prefix + b), 0) : 0;
     int key_lo, key_hi;
     reach_of(p, first, last, pre, kn, key_lo, key_hi);
-    int t0 = key_lo / kMmaKeys, t1 = (max(key_hi, key_lo) + kMmaKeys - 1) / kMmaKeys;
+    int t0 = key_lo / kMmaKeys, t1 = (key_hi + kMmaKeys - 1) / kMmaKeys;
     const int per = (t1 - t0 + P.nsplit - 1) / P.nsplit;
     t0 = min(t0 + split * per, t1);
     t1 = min(t0 + per, t1);

@@ -185,7 +185,8 @@ template <int KT> __device__ __forceinline__ void document_range(const int *ids,
     }
 }
 
-// Keys [lo, hi) that some query standing from `first` to `last` sees.
+// Keys [lo, hi) that some query standing from `first` to `last` sees; [0, 0) where there is none (queries that
+// stand a window past the last key).
 __device__ __forceinline__ void reach_of(const AttnDev &p, int first, int last, int pre, int kn, int &lo, int &hi)
 {
     lo = p.left == INT_MAX / 2 ? 0 : max(first - p.left, 0);
@@ -194,6 +195,7 @@ __device__ __forceinline__ void reach_of(const AttnDev &p, int first, int last, 
         lo = 0;
         hi = max(hi, min(pre, kn));
     }
+    if (lo >= hi) lo = hi = 0;
 }
 
 template <int DP, bool KEYS> struct MmaCfg {
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
     const int pre = p.prefix ? __ldg(p.prefix + b) : 0;
     int key_lo, key_hi;
     reach_of(p, first, last, pre, kn, key_lo, key_hi);
-    int t0 = key_lo / kMmaKeys, t1 = (max(key_hi, key_lo) + kMmaKeys - 1) / kMmaKeys;
+    int t0 = key_lo / kMmaKeys, t1 = (key_hi + kMmaKeys - 1) / kMmaKeys;
     if (KEYS && P.nsplit > 1) {
         const int per = (t1 - t0 + P.nsplit - 1) / P.nsplit;
         t0 = min(t0 + split * per, t1);
