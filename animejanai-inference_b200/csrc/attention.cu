@@ -218,7 +218,7 @@ bool check(const ajib_attn *op)
     if (op->left < -1 || op->right < -1) return false;
     if (misaligned4(op->q_len) || misaligned4(op->k_len) || misaligned4(op->prefix)) return false;
     if (misaligned4(op->q_doc) || misaligned4(op->k_doc) || misaligned4(op->bias_data)) return false;
-    if (!op->q_doc != !op->k_doc) return false;
+    if (op->lk && !op->q_doc != !op->k_doc) return false;  // (no keys: no ids of theirs)
     if (op->q_doc && (op->doc_rows < 1 || op->lk > 1 << 22)) return false;
     if (op->bias < AJIB_BIAS_NONE || op->bias > AJIB_BIAS_TABLE) return false;
     if (op->bias != AJIB_BIAS_NONE && !op->bias_data) return false;

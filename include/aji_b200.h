@@ -435,7 +435,7 @@ AJIB_EXPORT int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const aji
  * align_end).
  *
  * d is 1..256; lq and lk are up to 2^29 each (documents: lk up to 2^22). Zero batch or lq do
- * nothing; with lk 0 every query gets zeros. Outputs overlap no input. */
+ * nothing; with lk 0 every query gets zeros, and k, v and k_doc are not looked at. Outputs overlap no input. */
 enum ajib_bias { AJIB_BIAS_NONE = 0, AJIB_BIAS_SLOPE = 1, AJIB_BIAS_TABLE = 2 };
 typedef struct ajib_attn {
     int dtype; /* enum ajib_dtype */
