@@ -213,8 +213,9 @@ __device__ __forceinline__ bool item_of(const AttnDev &p, int b, int h, int tile
     x.before = (pre + KT - 1) / KT;
     x.before_whole = pre / KT;
     x.full = x.kn / KT;
-    x.t0 = x.before ? 0 : x.both ? min(x.from0, x.from1) : x.from0;
     x.t1 = max(max(x.before, x.to0), x.to1);
+    // (no further: queries that stand a window past the last key reach none, and the bit sets begin at t0)
+    x.t0 = min(x.before ? 0 : x.both ? min(x.from0, x.from1) : x.from0, x.t1);
     x.word0 = x.t0 / 32;
     return true;
 }

@@ -34,3 +34,14 @@ def test_queries_past_a_window(lq, lk, d):
         if "prefix" not in kw:
             assert (out[:, lk + 41:] == 0).all()
     run(*make("bf16", 2, lq, lk, 4, 4, d), left=3, k_len=[0, lk])
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("lq,lk", [(300, 70), (20000, 100), (70000, 4200)])
+def test_documents_of_queries_past_a_window(lq, lk, d):
+    """Far more queries than keys, a window and documents: items without a key tile, the documents' tiles
+    starting where the keys end."""
+    q, k, v = make("f16", 1, lq, lk, 2, 2, d)
+    out = run(q, k, v, left=5, q_doc=ids(lq, 1000), k_doc=ids(lk, 1000))
+    assert (out[:, lk + 6:] == 0).all()
+    run(q, k, v, left=5, prefix=[70], q_doc=ids(lq, 1 << 20), k_doc=ids(lk, 1 << 20))
