@@ -1,6 +1,6 @@
 /*
  * attention.cuh — what the attention kernels share: the arguments, which keys a query sees, the
- * score, and one row of attention by one warp.
+ * score, and the warp's matrix instruction.
  *
  * With scores s_j over the keys a query sees, out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m) for
  * any m; the kernels keep m = the running maximum and rescale sums by e^(m_old - m_new) when it
@@ -134,60 +134,37 @@ __device__ __forceinline__ float score2(const AttnDev &p, const Query &r, int j,
     return s;
 }
 
-// One query of one head over keys [j0, j1), by one warp: the maximum m, the sum l and the
-// unnormalised outputs, o[e] for component lane + 32 e. qs: kMaxHeadDim floats of shared memory of
-// this warp. Keys and values that the query does not see are not read. A lane takes a key for the
-// scores, a component for the values.
-template <typename T>
-__device__ void attend_row(const AttnDev &p, int b, int h, int i, int qn, int kn, int j0, int j1, float *qs, float &m,
-                           float &l, float (&o)[8])
-{
-    const int lane = threadIdx.x & 31, g = h / p.group;
-    const T *q = (const T *)p.q + b * p.qb + i * p.qt + h * p.qh;
-    const T *k = (const T *)p.k + b * p.kb + g * p.kh, *v = (const T *)p.v + b * p.vb + g * p.vh;
-    for (int e = lane; e < p.d; e += 32) qs[e] = to_f(q[e]);
-    __syncwarp();
-    const Query r = query_of(p, b, h, i, qn, kn);
-    const int *docs = p.k_doc ? p.k_doc + (int64_t)(b % p.doc_rows) * p.lk : nullptr;
-    m = -INFINITY;
-    l = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; e++) o[e] = 0.f;
-    j1 = min(j1, kn);
-    for (int jt = j0; jt < j1; jt += 32) {
-        const int j = jt + lane;
-        const bool seen = j < j1 && in_reach(r, j) && (!docs || __ldg(docs + j) == r.doc);
-        const unsigned any = __ballot_sync(0xffffffffu, seen);
-        if (!any) continue;
-        float s = -INFINITY;
-        if (seen) {
-            const T *kj = k + j * p.kt;
-            float dot = 0.f;
-            for (int e = 0; e < p.d; e++) dot = fmaf(qs[e], to_f(kj[e]), dot);
-            s = score2(p, r, j, dot);
-        }
-        float top = s;
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        top = fmaxf(top, m);
-        const float base = top == -INFINITY ? 0.f : top, alpha = exp2_fast(m - base);
-        m = top;
-        const float e2 = seen ? exp2_fast(s - base) : 0.f;
-        float sum = e2;
-        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        l = l * alpha + sum;
-#pragma unroll
-        for (int e = 0; e < 8; e++) o[e] *= alpha;
-        for (int c = 0; c < 32; c++) {
-            if (!(any >> c & 1)) continue;
-            const float w = __shfl_sync(0xffffffffu, e2, c);
-            const T *vj = v + (jt + c) * p.vt;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (lane + 32 * e < p.d) o[e] = fmaf(w, to_f(vj[lane + 32 * e]), o[e]);
-        }
+template <typename T> struct MmaOp;
+template <> struct MmaOp<__half> {
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+    {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
-    __syncwarp();
-}
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi)
+    {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ bool odd(uint32_t x) { return (x & 0x7c00u) == 0x7c00u; }  // not finite
+};
+template <> struct MmaOp<__nv_bfloat16> {
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+    {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi)
+    {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ bool odd(uint32_t x) { return (x & 0x7f80u) == 0x7f80u; }
+};
 
 }  // namespace dev
 }  // namespace ajib

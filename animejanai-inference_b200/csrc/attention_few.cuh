@@ -25,8 +25,7 @@ template <int DP> struct FewCfg {
     static constexpr int HALF = kMmaKeys * 128;        // 64 components of a tile's keys
     static constexpr int TILE = kMmaKeys * DP * 2, STAGE = 2 * TILE;
     static constexpr int RING = 16 * DP * 2;           // behind the queries (a multiple of 1024 bytes)
-    static constexpr int SCRATCH = RING + ST * STAGE;  // attend_row's queries, a warp each
-    static constexpr int BARS = SCRATCH + 4 * 256 * 4;
+    static constexpr int BARS = RING + ST * STAGE;
     static constexpr int SMEM = BARS + 2 * ST * 8 + 1024;
     static constexpr int BLOCKS = DP == 64 ? 3 : DP == 128 ? 2 : 1;
     static_assert(4 * 16 * (DP + 2) * 4 <= ST * STAGE, "the join reuses the ring");
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<DP>::BLOCKS)
     __syncthreads();  // the copies have landed and are read: the ring is free
     if (warp < 4) {
         join_warps<T, DP>(P, b, hk, row0, rows, split, qn, kn, t0 * kMmaKeys, min(t1 * kMmaKeys, kn), o, m, l,
-                          (float *)(sm + C::RING), (float *)(sm + C::SCRATCH) + warp * 256);
+                          (float *)(sm + C::RING));
     }
 }
 

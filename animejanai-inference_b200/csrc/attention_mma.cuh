@@ -14,6 +14,7 @@
 #pragma once
 
 #include "attention.cuh"
+#include "attention_odd.cuh"
 #include "sm100.cuh"
 
 namespace ajib {
@@ -67,36 +68,6 @@ __device__ __forceinline__ bool elect_one()
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
     return r != 0;
 }
-template <typename T> struct MmaOp;
-template <> struct MmaOp<__half> {
-    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-    {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ uint32_t pack(float lo, float hi)
-    {
-        uint32_t r;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-        return r;
-    }
-};
-template <> struct MmaOp<__nv_bfloat16> {
-    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-    {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ uint32_t pack(float lo, float hi)
-    {
-        uint32_t r;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-        return r;
-    }
-};
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -205,9 +176,8 @@ template <int DP, bool KEYS> struct MmaCfg {
     static constexpr int TILE = kMmaKeys * DP * 2;
     static constexpr int META = 3 * kMmaKeys * 4;  // documents, rows, columns of a tile's keys
     static constexpr int STAGE = 2 * TILE + META;
-    static constexpr int ROW_SCRATCH = 4 * 256 * 4;  // attend_row's queries
     static constexpr int JOIN = 4 * 16 * (DP + 2) * 4;
-    static constexpr int BITS = Q_BYTES + NST * STAGE + ROW_SCRATCH;
+    static constexpr int BITS = Q_BYTES + NST * STAGE;
     static_assert(!KEYS || JOIN <= NST * STAGE, "the join reuses the stages");
     // bits: two words (seen, whole) for every 32 tiles when there are documents
     static int smem(const AttnDev &p)
@@ -219,11 +189,11 @@ template <int DP, bool KEYS> struct MmaCfg {
 
 // Joins the results of four warps (threads 0 to 127) over keys of their own for the same 16 rows, in
 // memory of 4 * 16 * (DP + 2) floats, and writes them out, or to the workspace where the keys are
-// split. Rows that are not finite are taken again from the keys [j_begin, j_end) that they see.
+// split. Rows that are not finite are looked into (attention_odd.cuh): keys [j_begin, j_end), 16 a warp.
 template <typename T, int DP>
 __device__ __forceinline__ void join_warps(const MmaDev &P, int b, int hk, int row0, int rows, int split, int qn, int kn,
                                            int j_begin, int j_end, const float (&o)[DP / 8][4], const float (&m)[2],
-                                           const float (&l)[2], float *memory, float *scratch)
+                                           const float (&l)[2], float *memory)
 {
     const AttnDev &p = P.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -241,43 +211,63 @@ __device__ __forceinline__ void join_warps(const MmaDev &P, int b, int hk, int r
                 make_float2(o[n][2 * x], o[n][2 * x + 1]);
     }
     named_bar_sync(1, 128);
-    for (int r = warp; r < 16 && row0 + r < rows; r += 4) {
-        const int row = row0 + r, i = row / p.group, h = hk * p.group + row - i * p.group;
-        float top = -INFINITY, sum = 0.f, ro[8], f[4];
+    uint32_t left = 15;  // rows warp + 4 y to write
+    for (bool again = p.masked;; again = false) {
+        uint32_t odd_rows = 0;
+        for (int y = 0; y < 4 && row0 + warp + 4 * y < rows; y++) {
+            if (!(left >> y & 1)) continue;
+            const int r = warp + 4 * y, row = row0 + r, i = row / p.group, h = hk * p.group + row - i * p.group;
+            float top = -INFINITY, sum = 0.f, ro[8], f[4];
 #pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, jm[w * 16 + r]);
+            for (int w = 0; w < 4; w++) top = fmaxf(top, jm[w * 16 + r]);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            f[w] = exp2_fast(jm[w * 16 + r] - (top == -INFINITY ? 0.f : top));
-            sum += jl[w * 16 + r] * f[w];
-        }
-        bool odd = false;
+            for (int w = 0; w < 4; w++) {
+                f[w] = exp2_fast(jm[w * 16 + r] - (top == -INFINITY ? 0.f : top));
+                sum += jl[w * 16 + r] * f[w];
+            }
+            bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int c = lane + 32 * e;
-            ro[e] = 0.f;
-            if (c < p.d) {
+            for (int e = 0; e < 8; e++) {
+                const int c = lane + 32 * e;
+                ro[e] = 0.f;
+                if (c < p.d) {
 #pragma unroll
-                for (int w = 0; w < 4; w++) ro[e] += jo[(w * 16 + r) * DP + c] * f[w];
-                odd |= !(fabsf(ro[e]) < INFINITY);
+                    for (int w = 0; w < 4; w++) ro[e] += jo[(w * 16 + r) * DP + c] * f[w];
+                    odd |= !(fabsf(ro[e]) < INFINITY);
+                }
+            }
+            if (again && __any_sync(0xffffffffu, odd)) {
+                odd_rows |= 1u << y;
+                continue;
+            }
+            if (P.nsplit > 1) {
+                const int64_t slot = (((int64_t)b * p.hk + hk) * P.rows + row) * P.nsplit + split;
+                if (lane == 0) P.part_ml[slot] = make_float2(top, sum);
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (lane + 32 * e < p.d) P.part[slot * p.d + lane + 32 * e] = ro[e];
+            } else {
+                T *dst = (T *)p.out + b * p.ob + i * p.ot + h * p.oh;
+                const float g = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (lane + 32 * e < p.d) dst[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : ro[e] * g);
             }
         }
-        if (p.masked && __any_sync(0xffffffffu, odd))
-            attend_row<T>(p, b, h, i, qn, kn, j_begin, j_end, scratch, top, sum, ro);
-        if (P.nsplit > 1) {
-            const int64_t slot = (((int64_t)b * p.hk + hk) * P.rows + row) * P.nsplit + split;
-            if (lane == 0) P.part_ml[slot] = make_float2(top, sum);
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (lane + 32 * e < p.d) P.part[slot * p.d + lane + 32 * e] = ro[e];
-        } else {
-            T *dst = (T *)p.out + b * p.ob + i * p.ot + h * p.oh;
-            const float g = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (lane + 32 * e < p.d) dst[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : ro[e] * g);
+        if (!again || !named_bar_any(1, 128, odd_rows != 0)) break;
+        left = odd_rows;
+        const OddRows these = {b, hk * p.group, p.group, row0, rows, qn, kn};
+        if (named_bar_any(1, 128, unseen_odd<T>(p, these, j_begin + 32 * warp, j_end, 128))) {
+            redo_share<T, DP>(p, these, j_begin + 16 * warp, j_end, jm + warp * 16, jl + warp * 16, jo + warp * 16 * DP);
+            named_bar_sync(1, 128);
         }
     }
+}
+
+// (a call: inlined it costs the kernel's loops registers)
+template <typename T, int DP> __device__ __noinline__ void redo_rows_apart(const AttnDev &p, const OddRows &r, int j0, int j1)
+{
+    redo_rows<T, DP>(p, r, j0, j1);
 }
 
 template <typename T, int DP, bool KEYS>
@@ -289,7 +279,6 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
     const uint32_t sm0 = smem_u32(sm);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     char *const stage0 = sm + C::Q_BYTES;
-    float *const scratch = (float *)(sm + C::Q_BYTES + C::NST * C::STAGE) + warp * 256;
     uint32_t *const bits = (uint32_t *)(sm + C::BITS);
 
     // ---- which rows and keys ----
@@ -576,21 +565,13 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
     const int j_begin = t0 * kMmaKeys, j_end = min(t1 * kMmaKeys, kn);
 
     if (!KEYS) {
-        // A row whose result is not finite is taken again from the keys it sees alone: 0 * v of a key
-        // that it does not see is NaN when v is not finite.
-        uint32_t again = 0;
+        // rows that are not finite (attention_odd.cuh)
+        bool odd = false;
         if (p.masked) {
-            bool odd[2] = {false, false};
 #pragma unroll
             for (int n = 0; n < DP / 8; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) odd[e >> 1] |= !(fabsf(o[n][e]) < INFINITY);
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                uint32_t w = __ballot_sync(0xffffffffu, odd[x]);
-                for (int r = 0; r < 8; r++)
-                    if (w >> (4 * r) & 15) again |= 1u << (r + 8 * x);
-            }
+                for (int e = 0; e < 4; e++) odd |= !(fabsf(o[n][e]) < INFINITY);
         }
         __syncwarp();
         char *const mine = sm;  // rows m0 .. m0 + 15 of the queries' tile: this warp's alone
@@ -605,21 +586,6 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
             }
         }
         __syncwarp();
-        for (; again; again &= again - 1) {
-            const int r = __ffs(again) - 1, row = row0 + m0 + r, i = row / p.group;
-            if (row >= rows) break;
-            float rm, rl, ro[8];
-            attend_row<T>(p, b, hk * p.group + row - i * p.group, i, qn, kn, j_begin, j_end, scratch, rm, rl, ro);
-            const float f = rl == 0.f ? 0.f : 1.f / rl;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = lane + 32 * e;
-                if (c < p.d)
-                    *reinterpret_cast<T *>(mine + tile_at<DP>(m0 + r, c >> 3) + (c & 7) * 2) =
-                        from_f<T>(rl == 0.f ? 0.f : ro[e] * f);
-            }
-            __syncwarp();
-        }
         T *const out = (T *)p.out + b * p.ob + (int64_t)hk * p.group * p.oh;
         const int per = P.wo == 16 ? 8 : P.wo == 4 ? 2 : 1, units = p.d / per;
         for (int idx = lane; idx < 16 * units; idx += 32) {
@@ -634,12 +600,16 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
             else
                 *dst = *reinterpret_cast<const T *>(src);
         }
+        if (__any_sync(0xffffffffu, odd)) {
+            __syncwarp();
+            redo_rows_apart<T, DP>(p, {b, hk * p.group, p.group, row0 + m0, rows, qn, kn}, j_begin, j_end);
+        }
         return;
     }
 
     // ---- KEYS: join the four warps, then finish or hand on this split ----
     __syncthreads();
-    join_warps<T, DP>(P, b, hk, row0, rows, split, qn, kn, j_begin, j_end, o, m, l, (float *)stage0, scratch);
+    join_warps<T, DP>(P, b, hk, row0, rows, split, qn, kn, j_begin, j_end, o, m, l, (float *)stage0);
 }
 
 constexpr int kMaxSplits = 128;

@@ -65,8 +65,7 @@ template <int DP> struct TcCfg {
     static constexpr int BLOCKS = DP == 64 ? 2 : 1;    // on an SM
     static constexpr int ST = DP == 64 ? 3 : 2;        // stages of keys and of values
     static constexpr int QTILE = 128 * DP * 2, TILE = KT * DP * 2, HALF = KT * 128;  // HALF: a tile's 64 components
-    static constexpr int Q = 0, K = 2 * QTILE, V = K + ST * TILE, SCRATCH = V + ST * TILE;
-    static constexpr int BARS = SCRATCH + 8 * 256 * 4;  // attend_row's queries, a warp each
+    static constexpr int Q = 0, K = 2 * QTILE, V = K + ST * TILE, BARS = V + ST * TILE;
     static constexpr int NBAR = 4 + 4 * ST + 6 + 4 + 4;
     static constexpr int COLUMNS = 2 * KT + 2 * DP;     // of TMEM: scores of both query tiles, then outputs
     // One block of 384 threads an SM: 168 registers, of which the softmax warps take 216 and the others 72.
@@ -319,6 +318,22 @@ template <int KT> __device__ __forceinline__ void document_tiles(const AttnDev &
     }
     x.t0 = min(t_first, x.t1);
     x.t1 = t_last + 1;
+}
+
+// Every item of the block again, 16 rows in turn to each of the eight softmax warps, where the output is not
+// finite (attention_odd.cuh).
+template <typename T, int DP> __device__ __forceinline__ void redo_items(const TcDev &P)
+{
+    constexpr int KT = TcCfg<DP>::KT;
+    TcWalk walk;
+    TcItem it;
+    walk.start(P);
+    while (walk.next<KT>(P, it))
+        for (int q = 0, row0 = it.row0 + (threadIdx.x >> 5) * 16; q < 2 && row0 < it.qn; q++, row0 += 128) {
+            // the key tiles of this query tile
+            const int from = it.before ? 0 : q ? it.from1 : it.from0, to = max(it.before, q ? it.to1 : it.to0);
+            redo_rows<T, DP>(P.a, {it.b, it.h, 1, row0, it.qn, it.qn, it.kn}, from * KT, min(to * KT, it.kn));
+        }
 }
 
 template <typename T, int DP, int FORM>
@@ -581,14 +596,21 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
         // Two blocks an SM: 80 registers hold 32 scores of a row at a time, read twice. One: the whole row.
         constexpr bool TWICE = C::BLOCKS == 2;
         constexpr int CH = 32, W = TWICE ? 32 : KT;
-        uint32_t s_phase = 0, o_phase = 0;
-        uint32_t meets = 0;
+        uint32_t phase = 0;  // of s_full (bit 0), o_full (1) and meet (2)
+        bool odd_rows = false;  // whether a row of this thread came out not finite
         auto together = [&]() {  // the four warps of this query tile (bounded, unlike bar.sync)
             __syncwarp();
             if (lane == 0) mbar_arrive(meet + 8 * q);
-            return tc_wait_warp(meet + 8 * q, meets++ & 1, P.err, 219);
+            const bool here = tc_wait_warp(meet + 8 * q, phase >> 2, P.err, 219);
+            phase ^= 4;
+            return here;
         };
-        for (; __all_sync(0xffffffffu, next()); turn++) {
+        // With 80 registers the item stays in shared memory: its two dozen numbers are needed now and then (2040
+        // windows 540 us, in registers 596). With 216 it is copied (8192-token prompt 258 us, from shared memory 270).
+        using Item = typename std::conditional<C::BLOCKS == 2, const TcItem &, const TcItem>::type;
+        auto here = [&]() { return (ok = tc_wait(item_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213)) && items[turn & 1].b >= 0; };
+        for (; __all_sync(0xffffffffu, here()); turn++) {
+            Item x = items[turn & 1];
             if (grid && table_h != x.h) {
                 if (!(ok = together())) break;  // nobody reads the last head's any more
                 const float *src = p.bias_data + (int64_t)x.h * (2 * p.reach_y + 1) * (2 * p.reach_x + 1);
@@ -605,13 +627,11 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
             const Query r = query_at(p, x.doc_row, x.h, min(i, x.qn - 1), x.shift, x.pre);
             const int *const docs = documents ? p.k_doc + (int64_t)x.doc_row * p.lk : nullptr;
             const float *const mine = table + (p.reach_y - r.y) * P.table_st + p.reach_x - r.x;
-            const int from = q ? x.from1 : x.from0, to = q ? x.to1 : x.to0, before = q && !x.both ? 0 : x.before;
-            const int whole_from = q ? x.whole_from1 : x.whole_from0, whole_to = q ? x.whole_to1 : x.whole_to0;
             float m = -INFINITY, l = 0.f;  // m: in the units of the scores; times sc it is base 2
             bool any = false;
             for (int t = x.t0; t < x.t1; t++) {
-                bool seen_here = t < before || (t >= from && t < to);
-                bool all = t < x.full && (t < x.before_whole || (t >= whole_from && t < whole_to));
+                bool seen_here = t < x.before ? !q || x.both : t >= (q ? x.from1 : x.from0) && t < (q ? x.to1 : x.to0);
+                bool all = t < x.full && (t < x.before_whole || (t >= (q ? x.whole_from1 : x.whole_from0) && t < (q ? x.whole_to1 : x.whole_to0)));
                 if (bits) {
                     const uint32_t word = bits[4 * (t / 32 - x.word0) + q], whole = bits[4 * (t / 32 - x.word0) + 2 + q];
                     seen_here = seen_here && (word >> (t & 31) & 1);
@@ -619,8 +639,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                 }
                 if (!seen_here) continue;
                 const int j0 = t * KT;
-                if (!(ok = tc_wait_warp(s_full + 8 * q, s_phase, P.err, 210))) break;
-                s_phase ^= 1;
+                if (!(ok = tc_wait_warp(s_full + 8 * q, phase & 1, P.err, 210))) break;
+                phase ^= 1;
                 tc_fence_after();
                 // Scores that are more than a scaled product are made in a first pass, CH columns at a time (a short
                 // loop: unrolled over the row its instructions are fetched anew every time), and put back.
@@ -784,19 +804,20 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                 if (lane == 0) mbar_arrive(p_full + 8 * q);
             }
             if (!ok) break;
+            T *const dst = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)i * p.ot;
+            const bool none = q && !x.both;
             __syncwarp();
             if (lane == 0) done();
 
             // ---- out: a thread a row ----
             if (any) {
-                if (!(ok = tc_wait_warp(o_full + 8 * q, o_phase, P.err, 211))) break;
-                o_phase ^= 1;
+                if (!(ok = tc_wait_warp(o_full + 8 * q, phase >> 1 & 1, P.err, 211))) break;
+                phase ^= 2;
                 tc_fence_after();
             }
-            if (q && !x.both) continue;
+            if (none) continue;
             // (what a query without keys has accumulated is 0 * v: not finite only where the row is taken again)
             const float f = l == 0.f ? 0.f : 1.f / l;
-            T *const dst = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)i * p.ot;
             bool odd = false;
             for (int c = 0; c < p.d; c += 32) {
                 float o[32];
@@ -848,21 +869,11 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                         if (c + y < p.d) dst[c + y] = from_f<T>(o[y]);
                 }
             }
-            // A row that is not finite again from the keys that it sees alone (0 * v of one that it does not see
-            // is NaN when v is not finite).
-            uint32_t again = p.masked ? __ballot_sync(0xffffffffu, there && odd) : 0u;
-            for (; again; again &= again - 1) {
-                const int row = x.row0 + 128 * q + (warp & 3) * 32 + __ffs(again) - 1;
-                float rm, rl, ro[8];
-                attend_row<T>(p, x.b, x.h, row, x.qn, x.kn, x.t0 * KT, min(x.t1 * KT, x.kn),
-                              (float *)(sm + C::SCRATCH) + warp * 256, rm, rl, ro);
-                const float rf = rl == 0.f ? 0.f : 1.f / rl;
-                T *const to = (T *)p.out + x.b * p.ob + x.h * p.oh + (int64_t)row * p.ot;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (lane + 32 * e < p.d) to[lane + 32 * e] = from_f<T>(rl == 0.f ? 0.f : ro[e] * rf);
-            }
+            odd_rows |= there && odd;
         }
+        // Rows that are not finite (attention_odd.cuh), when the block's items are done: nobody waits for these
+        // warps any more but the barrier at the end.
+        if (p.masked && named_bar_any(3, 256, odd_rows)) redo_items<T, DP>(P);
     }
     tc_fence_before();
     __syncthreads();

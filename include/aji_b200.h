@@ -425,7 +425,8 @@ AJIB_EXPORT int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const aji
  *   - j < prefix of the sequence (int32 [batch], NULL: none), or else
  *   - j <= p if causal, p - j <= left if left >= 0, and j - p <= right if right >= 0.
  * A query that sees nothing gets zeros. What keys and values hold that a query does not see
- * (infinities and NaN too) does not reach it.
+ * (infinities and NaN too) does not reach it. An infinite value that it sees makes its component infinite, or
+ * NaN where the key's probability is so small that it is held as 0.
  *
  * Bias, fp32 on the device: AJIB_BIAS_SLOPE adds -bias_data[h] * |p - j| (hq slopes);
  * AJIB_BIAS_TABLE adds a table's entry for the distance of the key from the query, clamped to the
