@@ -37,8 +37,9 @@ struct MmaDev {
 namespace dev {
 
 // mbar_wait with a hint (10 us) of how long the hardware may keep a waiting thread asleep: the roles of
-// this kernel wait for one another most of the time, and polling took their issue slots.
-__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err, int code)
+// this kernel wait for one another most of the time, and polling took their issue slots. tiles: how many key
+// tiles (at most 2.2 us each) may rightly come between, for which 40 us each are added to the 2 s.
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err, int code, int tiles = 0)
 {
     if (mbar_test_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer();
@@ -50,15 +51,15 @@ __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err,
             : "r"(bar), "r"(parity), "r"(10000u)
             : "memory");
         if (done) return true;
-        if (globaltimer() - t0 > 2000000000ull) {
+        if (globaltimer() - t0 > 2000000000ull + (uint64_t)tiles * 40000ull) {
             atomicCAS(err, 0, code);
             return false;
         }
     }
 }
-__device__ __forceinline__ bool tc_wait_warp(uint32_t bar, uint32_t parity, int *err, int code)
+__device__ __forceinline__ bool tc_wait_warp(uint32_t bar, uint32_t parity, int *err, int code, int tiles = 0)
 {
-    return __all_sync(0xffffffffu, tc_wait(bar, parity, err, code));
+    return __all_sync(0xffffffffu, tc_wait(bar, parity, err, code, tiles));
 }
 // One lane of a converged warp. (Told by a lane number instead, the compiler takes the operands of the
 // branch's products and copies for divergent, and each issue costs 140 cycles instead of a few.)

@@ -381,10 +381,11 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
     const bool documents = p.q_doc != nullptr;
     int turn = 0;  // items so far (their places in shared memory alternate)
     bool ok = true;
-    // The next item, from warp 11; done() gives its place back.
+    // The next item, from warp 11; done() gives its place back. (A wait for an item, or for the first scores of
+    // one, may be for as long as another takes: up to 2^29 keys. The other waits are for a tile.)
     TcItem x;
     auto next = [&]() {
-        if (!(ok = tc_wait(item_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213))) return false;
+        if (!(ok = tc_wait(item_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213, p.lk / KT))) return false;
         x = items[turn & 1];
         return x.b >= 0;
     };
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
             for (;; turn++) {
                 const bool more = walk.next<KT>(P, x);
                 if (!more) x.b = -1;
-                if (!tc_wait_warp(item_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214)) break;
+                if (!tc_wait_warp(item_empty + 8 * (turn & 1), (turn >> 1 & 1) ^ 1, P.err, 214, p.lk / KT)) break;
                 if (more && documents) document_tiles<KT>(p, x, bit_sets + (turn & 1) * P.words * 4);
                 if (lane == 0) items[turn & 1] = x;
                 __syncwarp();
@@ -606,9 +607,9 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
             return here;
         };
         // With 80 registers the item stays in shared memory: its two dozen numbers are needed now and then (2040
-        // windows 540 us, in registers 596). With 216 it is copied (8192-token prompt 258 us, from shared memory 270).
+        // windows 550 us, in registers 596). With 216 it is copied (8192-token prompt 258 us, from shared memory 270).
         using Item = typename std::conditional<C::BLOCKS == 2, const TcItem &, const TcItem>::type;
-        auto here = [&]() { return (ok = tc_wait(item_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213)) && items[turn & 1].b >= 0; };
+        auto here = [&]() { return (ok = tc_wait(item_full + 8 * (turn & 1), turn >> 1 & 1, P.err, 213, p.lk / KT)) && items[turn & 1].b >= 0; };
         for (; __all_sync(0xffffffffu, here()); turn++) {
             Item x = items[turn & 1];
             if (grid && table_h != x.h) {
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                 }
                 if (!seen_here) continue;
                 const int j0 = t * KT;
-                if (!(ok = tc_wait_warp(s_full + 8 * q, phase & 1, P.err, 210))) break;
+                if (!(ok = tc_wait_warp(s_full + 8 * q, phase & 1, P.err, 210, p.lk / KT))) break;
                 phase ^= 1;
                 tc_fence_after();
                 // Scores that are more than a scaled product are made in a first pass, CH columns at a time (a short
