@@ -89,11 +89,12 @@ __device__ __forceinline__ int position_of(const QkDev &p, int b, int t)
 }
 
 // A sum of squares that left the range of a float (bf16 heads near 1e19 and beyond, or tiny ones with
-// next to no eps) is taken again over values times this power of two. 1: the sum will do. (Below
-// 2^-80 against an eps of 2^-40 or more the sum does not matter.)
+// next to no eps) is taken again over values times this power of two (256 of the largest bf16 values
+// then sum to 2^104). 1: the sum will do. (Below 2^-80 against an eps of 2^-40 or more the sum does not
+// matter.)
 __device__ __forceinline__ float rescale_of(const QkDev &p, float sum)
 {
-    return sum > 3.4e38f ? 0x1p-64f : sum < 0x1p-80f && p.eps < 0x1p-40f ? 0x1p64f : 1.f;
+    return sum > 3.4e38f ? 0x1p-80f : sum < 0x1p-80f && p.eps < 0x1p-40f ? 0x1p64f : 1.f;
 }
 
 // What a head is multiplied by, from the sum of its squares times scale^2 (rsqrt: 2 ulp).
