@@ -89,20 +89,22 @@ __device__ __forceinline__ int position_of(const QkDev &p, int b, int t)
 }
 
 // A sum of squares that left the range of a float (bf16 heads near 1e19 and beyond, or tiny ones with
-// next to no eps) is taken again over values times this power of two (256 of the largest bf16 values
-// then sum to 2^104). 1: the sum will do. (Below 2^-80 against an eps of 2^-40 or more the sum does not
-// matter.)
+// next to no eps) is taken again over values times this power of two: 256 of the largest bf16 values
+// then sum to 2^104, one of the smallest to 2^-106. 1: the sum will do. (Below 2^-80 against an eps of
+// 2^-40 or more the sum does not matter.)
 __device__ __forceinline__ float rescale_of(const QkDev &p, float sum)
 {
-    return sum > 3.4e38f ? 0x1p-80f : sum < 0x1p-80f && p.eps < 0x1p-40f ? 0x1p64f : 1.f;
+    return sum > 3.4e38f ? 0x1p-80f : sum < 0x1p-80f && p.eps < 0x1p-40f ? 0x1p80f : 1.f;
 }
 
-// What a head is multiplied by, from the sum of its squares times scale^2 (rsqrt: 2 ulp).
+// What a head is multiplied by, from the sum of the squares of its values times scale (rsqrt: 2 ulp). A scale
+// above 1 stays in the values, as the factor of the values alone may pass a float's range.
 __device__ __forceinline__ float norm_factor(const QkDev &p, float sum, float scale)
 {
-    if (p.norm == AJIB_NORM_RMS) return scale * rsqrtf(sum * p.inv_d + p.eps * scale * scale);
-    const float f = scale * rsqrtf(sum);
-    return f > p.inv_eps ? p.inv_eps : f;  // not fminf, which drops a NaN
+    const float down = fminf(scale, 1.f);
+    if (p.norm == AJIB_NORM_RMS) return down * rsqrtf(sum * p.inv_d + p.eps * scale * scale);
+    const float f = down * rsqrtf(sum), most = scale > 1.f ? p.inv_eps * 0x1p-80f : p.inv_eps;
+    return f > most ? most : f;  // not fminf, which drops a NaN
 }
 
 // One warp per head of one token, any d, alignment and rotary dim: lane l owns pairs l, l + 32, ...
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ Q
     if (h >= p.t[0].heads) h -= p.t[0].heads;
     const T *src = (const T *)x.src + b * x.sb + t * x.st + h * x.sh;
     T *dst = (T *)x.dst + b * x.ob + t * x.ot + h * x.oh;
-    float f = 1.f;
+    float f = 1.f, up = 1.f;
     if (p.norm) {
         float sum, scale = 1.f;
         for (;;) {
@@ -135,12 +137,13 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ Q
             if (scale != 1.f || (scale = rescale_of(p, sum)) == 1.f) break;
         }
         f = norm_factor(p, sum, scale);
+        up = fmaxf(scale, 1.f);
     }
     const int npair = p.rot >> 1;
     const Place place = place_of(p, p.rot ? position_of(p, b, t) : 0);
     for (int i = lane; i < npair; i += 32) {
         const int i1 = p.interleaved ? 2 * i : i, i2 = p.interleaved ? 2 * i + 1 : i + npair;
-        float x1 = to_f(src[i1]) * f, x2 = to_f(src[i2]) * f, c, s;
+        float x1 = to_f(src[i1]) * up * f, x2 = to_f(src[i2]) * up * f, c, s;
         if (x.w) {
             x1 *= x.w[i1];
             x2 *= x.w[i2];
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_any(const __grid_constant__ Q
         dst[i2] = from_f<T>(x2 * c + x1 * s);
     }
     for (int i = p.rot + lane; i < p.d; i += 32) {
-        float v = to_f(src[i]) * f;
+        float v = to_f(src[i]) * up * f;
         if (x.w) v *= x.w[i];
         dst[i] = from_f<T>(v);
     }
@@ -336,6 +339,12 @@ __global__ void __launch_bounds__(kQkThreads, NORM ? (TURN ? 7 : 8) : 6) k_qk_ve
                     if (scale != 1.f) {  // (every lane of the head agrees)
                         sum = sum_squares<N>(a, e, scale);
                         for (int m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(all, sum, m);
+                        const float up = fmaxf(scale, 1.f);
+#pragma unroll
+                        for (int i = 0; i < N; i++) {
+                            a[i] = f2_mul(a[i], f2(up, up));
+                            e[i] = f2_mul(e[i], f2(up, up));
+                        }
                     }
                     const float f = norm_factor(p, sum, scale);
                     const F2 ff = f2(f, f);

@@ -33,3 +33,37 @@ def test_large_heads(value, which, d):
     x[0, 2, :, 1:] *= 1e-3
     for eps in (1e-6, 0.0):
         assert_qk(norm(x, which, eps), ref_qk(x, norm=which, eps=eps))
+
+
+@pytest.mark.parametrize("d", SIZES)
+@pytest.mark.parametrize("which", ["rms", "l2"])
+@pytest.mark.parametrize("value", [2.0 ** -133, 2.0 ** -130, 3e-39, 1e-37, 1e-30, 2.0 ** -41, 2.0 ** -40])
+def test_small_heads(value, which, d):
+    """Values down to bf16's smallest subnormal, with next to no eps: unit values, or what eps leaves of them."""
+    x = torch.full((1, 3, 2, d), 1.0, device="cuda").bfloat16() * value
+    x[0, 1, :, ::2] *= -1
+    x[0, 2, :, d // 2:] = 0
+    for eps in (0.0, 1e-37, 1e-20, 1e-13, 1e-6):
+        assert_qk(norm(x, which, eps), ref_qk(x, norm=which, eps=eps))
+
+
+@pytest.mark.parametrize("which", ["rms", "l2"])
+@pytest.mark.parametrize("layout", [0, 1])
+def test_extremes_that_turn(which, layout):
+    import ajib
+    rot = ajib.Rotary(64, layout=layout)
+    f = torch.tensor(rot.table()[0], dtype=torch.float64, device="cuda")
+    x = torch.randn(1, 6, 2, 64, device="cuda").bfloat16()
+    for t, by in enumerate([BF.max / 8, 1e30, 1.0, 1e-30, 1e-37, 0.0]):
+        x[0, t] = (x[0, t].double() * by).bfloat16()
+    angles = torch.arange(6, device="cuda").double()[None, :, None] * f
+    eps = 1e-30
+    want = ref_qk(x, norm=which, eps=eps, angles=angles, layout="half" if layout == 0 else "interleaved")
+    assert_qk(norm(x, which, eps, rot=rot), want)
+
+
+def test_fp16_ends():
+    x = torch.full((1, 2, 2, 64), 65504.0, device="cuda").half()
+    x[0, 1] = 2.0 ** -24
+    for which in ("rms", "l2"):
+        assert_qk(norm(x, which, 0.0), ref_qk(x, norm=which, eps=0.0))
