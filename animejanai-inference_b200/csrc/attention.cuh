@@ -57,9 +57,19 @@ __device__ __forceinline__ float rcp_fast(float x)
     return y;
 }
 
-// tanh to about 2^-22 of 1: 1 - 2 / (e^2x + 1). (The hardware's tanh.approx is good to 2^-11, which
-// a cap of 50 would turn into 0.02 of score, 2 % of a probability.)
-__device__ __forceinline__ float tanh_exp(float x) { return 1.f - 2.f * rcp_fast(exp2_fast(x * (2.f * kLog2e)) + 1.f); }
+// tanh to 2^-21 of itself, so that a score far below its cap is as good as one without: up to 0.75 an odd
+// polynomial of degree 11 (minimax fit of tanh(x) / x in x^2, relative error 3e-8), above it 1 - 2 / (e^2x + 1),
+// which cancels near 0. (A fit up to 1 of that error has degree 13: prompts under a cap 73 us for 70. The
+// hardware's tanh.approx is good to 2^-11, which a cap of 50 would turn into 0.02 of score, 2 % of a probability.)
+constexpr float kTanhTo = 0.75f;
+constexpr float kTanh0 = 0.999999971013924f, kTanh1 = -0.33332958879535546f, kTanh2 = 0.13325406018726102f,
+                kTanh3 = -0.05334443020680119f, kTanh4 = 0.01958290833624651f, kTanh5 = -0.004716257367942312f;
+__device__ __forceinline__ float tanh_of(float x)
+{
+    const float z = x * x, far = 1.f - 2.f * rcp_fast(exp2_fast(x * (2.f * kLog2e)) + 1.f);
+    const float y = fmaf(fmaf(fmaf(fmaf(fmaf(kTanh5, z, kTanh4), z, kTanh3), z, kTanh2), z, kTanh1), z, kTanh0);
+    return fabsf(x) <= kTanhTo ? y * x : far;
+}
 
 // How many queries / keys sequence b has.
 __device__ __forceinline__ int q_count(const AttnDev &p, int b)
@@ -125,7 +135,7 @@ __device__ __forceinline__ float table_bias(const AttnDev &p, const Query &r, in
 // The score of key j times log2(e), from its product with the query.
 __device__ __forceinline__ float score2(const AttnDev &p, const Query &r, int j, float dot)
 {
-    float s = p.cap_out > 0.f ? p.cap_out * tanh_exp(dot * p.cap_in) : dot * p.scale;
+    float s = p.cap_out > 0.f ? p.cap_out * tanh_of(dot * p.cap_in) : dot * p.scale;
     if (p.bias == AJIB_BIAS_SLOPE) s -= r.slope * (float)abs(r.at - j);
     if (p.bias == AJIB_BIAS_TABLE) {
         const int jy = p.grid_w ? j / p.grid_w : 0;

@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kMmaThreads) k_attn_mma(const __grid_constant_
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[n][e] = p.cap_out * tanh_exp(s[n][e] * p.cap_in);
+                for (int e = 0; e < 4; e++) s[n][e] = p.cap_out * tanh_of(s[n][e] * p.cap_in);
         } else {
 #pragma unroll
             for (int n = 0; n < NT; n++)

@@ -138,15 +138,15 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
-// tanh of two in [-1, 1] on the FMA pipe: odd polynomial of degree 11 (minimax fit, error 3e-7).
+// tanh of two in [-0.75, 0.75] (tanh_of's polynomial).
 __device__ __forceinline__ F2 f2_tanh(F2 x)
 {
     const F2 z = f2_mul(x, x);
-    F2 y = f2_fma(f2(-0.0028189276345074177f, -0.0028189276345074177f), z, f2(0.01605205424129963f, 0.01605205424129963f));
-    y = f2_fma(y, z, f2(-0.050903141498565674f, -0.050903141498565674f));
-    y = f2_fma(y, z, f2(0.1325000524520874f, 0.1325000524520874f));
-    y = f2_fma(y, z, f2(-0.33323246240615845f, -0.33323246240615845f));
-    y = f2_fma(y, z, f2(0.9999963641166687f, 0.9999963641166687f));
+    F2 y = f2_fma(f2(kTanh5, kTanh5), z, f2(kTanh4, kTanh4));
+    y = f2_fma(y, z, f2(kTanh3, kTanh3));
+    y = f2_fma(y, z, f2(kTanh2, kTanh2));
+    y = f2_fma(y, z, f2(kTanh1, kTanh1));
+    y = f2_fma(y, z, f2(kTanh0, kTanh0));
     return f2_mul(y, x);
 }
 
@@ -656,19 +656,19 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::BLOCKS)
                         tmem_wait_ld();
                         if (scaled) {
                             if (capped) {
-                                // exponentials and reciprocals of the tanh are three times the unit's work: below the cap a
-                                // polynomial does
+                                // where all scores are below 0.75 of the cap the polynomial does, without the other form's exponential and
+                                // reciprocal
                                 float far = 0.f;
 #pragma unroll
                                 for (int c = 0; c < CH; c += 2) far = max3(far, fabsf(s[c]), fabsf(s[c + 1]));
-                                if (__all_sync(0xffffffffu, far * fabsf(p.cap_in) <= 1.f)) {
+                                if (__all_sync(0xffffffffu, far * fabsf(p.cap_in) <= kTanhTo)) {
                                     const F2 in = f2(p.cap_in, p.cap_in), out = f2(p.cap_out, p.cap_out);
 #pragma unroll
                                     for (int c = 0; c < CH; c += 2)
                                         f2_out(f2_mul(f2_tanh(f2_mul(f2(s[c], s[c + 1]), in)), out), s[c], s[c + 1]);
                                 } else {
 #pragma unroll
-                                    for (int c = 0; c < CH; c++) s[c] = p.cap_out * tanh_exp(s[c] * p.cap_in);
+                                    for (int c = 0; c < CH; c++) s[c] = p.cap_out * tanh_of(s[c] * p.cap_in);
                                 }
                             } else if (FORM != kFormGrid && !(FORM == kFormAny && grid)) {
 #pragma unroll
