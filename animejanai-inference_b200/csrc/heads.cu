@@ -503,6 +503,7 @@ extern "C" int ajib_rotary_create(const ajib_rotary_params *p, ajib_rotary **out
             if (!std::isfinite(f[i])) return AJIB_ERR_ARGS;
     }
     if (p->amplitude > 0) amp = p->amplitude;
+    if (!(amp > 0) || !std::isfinite((float)amp)) return AJIB_ERR_ARGS;  // (BANDS with a factor below e^-10)
     ajib_rotary *r = new (std::nothrow) ajib_rotary;
     if (!r) return AJIB_ERR_NO_MEM;
     r->dim = p->dim;

@@ -361,8 +361,10 @@ typedef struct ajib_heads {
  *   AJIB_ROTARY_BANDS   frequencies that turn more than beta_fast times over `trained` positions
  *                       stay, those that turn less than beta_slow times are divided by factor, a
  *                       ramp over i between; beta 0: 32 and 1 (published as YaRN). The turned
- *                       components are also scaled by 1 + 0.1 ln(factor) unless amplitude is given.
- * amplitude: what the turned components are multiplied by; 0: 1, or the BANDS value.
+ *                       components are also scaled by 1 + 0.1 ln(factor) unless amplitude is given (the
+ *                       published form keeps 1 for factors below 1).
+ * amplitude: what the turned components are multiplied by; 0: 1, or the BANDS value, which is refused
+ * where it is not positive (a factor of e^-10 or less).
  * freq: NULL, or dim / 2 / axes angles per position (radians, finite, not negative) that replace
  * base and scaling. */
 enum ajib_rotary_layout { AJIB_ROTARY_HALF = 0, AJIB_ROTARY_INTERLEAVED = 1 };

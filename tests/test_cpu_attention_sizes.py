@@ -1,4 +1,8 @@
 """CPU: arguments of the attention operators at the edges of their ranges."""
+import math
+
+import pytest
+
 ARGS = -2
 P = 0x10000  # an address that nothing looks at
 
@@ -10,3 +14,18 @@ def test_documents_without_keys():
     q = ajib.heads(P, 1280, 256, 64)
     assert ajib.attention(op(0), q, None, None, q) == 0
     assert ajib.attention(op(3), q, q, q, q) == ARGS
+
+
+def test_amplitudes():
+    """What turned components are multiplied by is positive, and a float: with a factor below e^-10 the stretched
+    bands' 1 + 0.1 ln(factor) is not."""
+    import ajib
+    bands = lambda factor, **kw: ajib.Rotary(64, scaling=ajib.ROTARY_BANDS, factor=factor, trained=4096, **kw)
+    for factor in (math.exp(-10.5), 1e-5, 1e-300):
+        with pytest.raises(ajib.AjibError):
+            bands(factor)
+        assert bands(factor, amplitude=1.0).table()[1] == 1.0
+    assert math.isclose(bands(math.exp(-9.5)).table()[1], 0.05, rel_tol=1e-9)
+    for amplitude in (1e39, 1e300):
+        with pytest.raises(ajib.AjibError):
+            ajib.Rotary(64, amplitude=amplitude)
