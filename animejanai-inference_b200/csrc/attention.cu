@@ -47,6 +47,14 @@ size_t packed_bytes(const ajib_attn *op, int dp, int tensor)
     return (size_t)op->batch * (tensor ? (size_t)op->lk * op->hk : (size_t)op->lq * op->hq) * dp * 2;
 }
 
+// Whether the copies are of a size that a device may hold (of repeated sequences they need not be, and the
+// number of their bytes may pass 64 bits).
+bool packable(const ajib_attn *op, int dp)
+{
+    const __int128 most = std::max((__int128)op->lk * op->hk, (__int128)op->lq * op->hq);
+    return most * op->batch * dp * 2 <= (__int128)1 << 42;
+}
+
 // Which kernel. Measured (us, 8 heads, causal; k_attn_mma / few / tc):
 //   64 components, 200 tokens 12.3 / 9.0 / 14.4, 800 26 / 18 / 27; 16 sequences of 150 20 / 23 / 14
 //   128 components, 500 tokens 27 / 14 / 19, 800 39 / 27 / 21
@@ -75,8 +83,10 @@ bool choose(const ajib_attn *op, Choice &c)
         const bool grid = op->bias == AJIB_BIAS_TABLE && op->grid_w;
         c.tc = (!grid || grid_reached(op)) && (int64_t)op->batch * op->hq * ((op->lq + 255) / 256) <= 0x7fffffff &&
                (op->d <= 64 ? TcCfg<64>::smem(op) : TcCfg<128>::smem(op)) <= kMaxSmem;
-        if (c.tc && op->d % 8) {
-            c.pack = (op->d + 7) / 8 * 8;
+        const int dp = (op->d + 7) / 8 * 8;
+        c.tc = c.tc && (op->d == dp || packable(op, dp));
+        if (c.tc && op->d != dp) {
+            c.pack = dp;
             for (int i = 0; i < 3; i++) c.space += packed_bytes(op, c.pack, i);
         }
     }

@@ -29,3 +29,15 @@ def test_amplitudes():
     for amplitude in (1e39, 1e300):
         with pytest.raises(ajib.AjibError):
             ajib.Rotary(64, amplitude=amplitude)
+
+
+def test_workspace_of_repeated_sequences():
+    """Keys that every sequence shares (stride 0) may be more, taken one by one, than 64 bits of bytes: no workspace
+    for copies of them is asked for, where its size came out as that of the queries' copies alone."""
+    import ajib
+    for batch, hk, lk in ((1 << 20, 1 << 10, 1 << 29), (1 << 19, 1 << 10, 1 << 29), (1 << 16, 1 << 6, 1 << 29)):
+        op = ajib.attn_op(ajib.F16, batch, 32, lk, hk, hk, 7, 0.125)
+        assert ajib.attention_workspace(op) == 0
+    # ordinary ones still are packed: queries, keys and values in rows of 32 components
+    op = ajib.attn_op(ajib.F16, 60, 200, 100, 6, 6, 30, 0.125)
+    assert ajib.attention_workspace(op) == 60 * (200 + 2 * 100) * 6 * 32 * 2
