@@ -118,7 +118,7 @@ cudaError_t run_few(const MmaDev &p, const CUtensorMap (&m)[3], cudaStream_t s)
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(k_attn_few<T, DP>, kMaxSmem, done);
     if (e != cudaSuccess) return e;
-    int *const err = attn_status_word();
+    int *const err = status_word();
     if (!err) return cudaErrorUnknown;
     const int64_t blocks = (int64_t)p.a.batch * p.a.hk * p.row_tiles * p.nsplit;
     k_attn_few<T, DP><<<(unsigned)blocks, kFewThreads, FewCfg<DP>::SMEM, s>>>(p, m[1], m[2], err);
@@ -244,16 +244,6 @@ bool check(const ajib_attn *op)
 }  // namespace
 }  // namespace ajib
 
-// The attention kernels' status word: of this library's image on the device, so that a first launch
-// needs no allocation and can be captured. ajib_kernel_status reads it with the convolutions'.
-__device__ int g_attn_status;
-
-int *ajib::attn_status_word()
-{
-    void *p = nullptr;
-    return cudaGetSymbolAddress(&p, g_attn_status) == cudaSuccess ? (int *)p : nullptr;
-}
-
 using namespace ajib;
 
 extern "C" size_t ajib_attention_workspace(const ajib_attn *op)
@@ -372,7 +362,7 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
         const uint64_t rows = (uint64_t)(uintptr_t)out->p | (uint64_t)d * 2 | (uint64_t)(b > 1 ? out->sb : 0) * 2 |
                               (uint64_t)out->st * 2 | (uint64_t)(op->hq > 1 ? out->sh : 0) * 2;
         t.wo = rows % 32 == 0 ? 32 : m.wo;
-        t.err = attn_status_word();
+        t.err = status_word();
         if (!t.err) return AJIB_ERR_CUDA;
         const cudaError_t e = op->dtype == AJIB_F16 ? attn_tc_f16(t, op, maps, (cudaStream_t)stream)
                                                     : attn_tc_bf16(t, op, maps, (cudaStream_t)stream);

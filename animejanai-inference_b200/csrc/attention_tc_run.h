@@ -13,8 +13,8 @@
 
 namespace ajib {
 
-int sm_count();           // conv.cu
-int *attn_status_word();  // attention.cu
+int sm_count();      // conv.cu
+int *status_word();  // conv.cu
 
 constexpr int kMaxSmem = 227 * 1024;
 

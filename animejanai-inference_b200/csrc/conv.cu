@@ -37,8 +37,6 @@ struct ajib_weights {
 
 namespace ajib {
 
-int *attn_status_word();  // attention.cu
-
 int pad_k(int cin) { return cin <= 16 ? 16 : (cin + 15) / 16 * 16; }
 // 3x3 outputs pad to 16, 32, 48 or 64 columns. 48 channels (SPAN, SPANF3) keep their width: a
 // row's stacked-tap MMA is then N = 144 rather than 192 (a quarter fewer tensor cycles), and the
@@ -72,8 +70,10 @@ std::vector<uint16_t> pack_b_image(const uint16_t *w, int taps, int cin, int cou
     return img;
 }
 
-// ---- per-device status word (kernels record pipeline timeouts here) ----
+// ---- per-device status word (kernels record pipeline timeouts here): of this library's image on the
+// device, so that a first launch needs no allocation and can be captured ----
 namespace {
+__device__ int g_status_word;
 std::mutex g_status_mu;
 int *g_status[64] = {};
 }  // namespace
@@ -83,16 +83,9 @@ int *status_word()
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lk(g_status_mu);
-    if (!g_status[dev]) {
-        int *p = nullptr;
-        if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-        if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) {
-            cudaFree(p);
-            return nullptr;
-        }
-        g_status[dev] = p;
-    }
-    return g_status[dev];
+    void *p = g_status[dev];
+    if (!p && cudaGetSymbolAddress(&p, g_status_word) != cudaSuccess) return nullptr;
+    return g_status[dev] = (int *)p;
 }
 
 int sm_count()
@@ -599,15 +592,12 @@ extern "C" size_t ajib_feature_bytes(int H, int W, int C)
 
 extern "C" int ajib_kernel_status(int clear)
 {
-    int first = 0;
-    for (int *w : {status_word(), attn_status_word()}) {
-        if (!w) return AJIB_ERR_CUDA;
-        int v = 0;
-        if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return AJIB_ERR_CUDA;
-        if (clear && v && cudaMemset(w, 0, sizeof(int)) != cudaSuccess) return AJIB_ERR_CUDA;
-        if (!first) first = v;
-    }
-    return first;
+    int *w = status_word();
+    if (!w) return AJIB_ERR_CUDA;
+    int v = 0;
+    if (cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return AJIB_ERR_CUDA;
+    if (clear && v && cudaMemset(w, 0, sizeof(int)) != cudaSuccess) return AJIB_ERR_CUDA;
+    return v;
 }
 
 // ---- the model input packed into a strip-chunked map (the executor's head path) ----
