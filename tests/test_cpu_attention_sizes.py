@@ -41,3 +41,25 @@ def test_workspace_of_repeated_sequences():
     # ordinary ones still are packed: queries, keys and values in rows of 32 components
     op = ajib.attn_op(ajib.F16, 60, 200, 100, 6, 6, 30, 0.125)
     assert ajib.attention_workspace(op) == 60 * (200 + 2 * 100) * 6 * 32 * 2
+
+
+@pytest.mark.parametrize("dim,axes,base,trained,fast,slow,factor", [
+    (128, 1, 10000.0, 2048, 0, 0, 8.0), (64, 1, 10000.0, 4096, 0, 0, 16.0), (64, 1, 500000.0, 8192, 32, 1, 4.0),
+    (96, 1, 10000.0, 100, 8, 2, 2.0), (64, 2, 10000.0, 4096, 0, 0, 4.0), (128, 1, 10000.0, 3, 0, 0, 8.0)])
+def test_ramp_of_bands(dim, axes, base, trained, fast, slow, factor):
+    """Every frequency, the ramp's too: between the pairs that turn `fast` and `slow` times over the trained
+    positions (whole pairs, outwards) the part of f / factor rises evenly from 0 to 1."""
+    import ajib
+    got, _ = ajib.Rotary(dim, axes=axes, grid_w=30 if axes == 2 else 0, base=base, scaling=ajib.ROTARY_BANDS, factor=factor,
+                         trained=trained, beta_fast=fast, beta_slow=slow).table()
+    n = dim // axes
+    # pair i turns trained * base^(-2 i / n) / (2 pi) times
+    where = lambda turns: n / 2 * math.log(trained / (2 * math.pi * turns), base)
+    lo, hi = max(0, math.floor(where(fast or 32))), min(n - 1, math.ceil(where(slow or 1)))
+    ramps = 0
+    for i, f in enumerate(got):
+        plain = base ** (-2 * i / n)
+        part = min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001)))
+        ramps += 0 < part < 1
+        assert math.isclose(f, plain * (1 - part) + plain / factor * part, rel_tol=1e-12), i
+    assert len(got) == n // 2 and (ramps or trained == 3)
