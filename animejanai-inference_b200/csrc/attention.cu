@@ -61,11 +61,11 @@ bool packable(const ajib_attn *op, int dp)
 // so few while all its blocks run at once, then tc: 600 windows of 144 tokens of 6 heads 303 / 723 / 169, 464
 // windows of 64 of 3 heads - / 97 / 27 (below kTcQueries few again, whose blocks hold 16 rows).
 // Heads of a size that TMA cannot copy (d not a multiple of 8) are copied to padded rows for tc.
-// With few queries the keys are also split until there is a block an SM (three where lengths are given,
-// which makes caches uneven) or a split has only kSplitTiles tiles. (us, with one / two / three blocks an
-// SM: 2 x 16384 keys of 8 heads of 128 33 / 37 / 39; 8 caches of 9 to 16 thousand keys 78 / 79 / 75, five
-// tokens over them 102 / 97 / 89; with at least 4 / 8 tiles a split: 4000 keys 14.2 / 16.4, 1500 keys
-// 12.4 / 13.9.)
+// With few queries the keys are also split until there is a block an SM, or a split has only kSplitTiles tiles of
+// all the keys (a window leaves it fewer, and some splits none). Three blocks an SM where lengths are given: caches
+// are then uneven as a rule, 8 of 9 to 16 thousand keys take 78 / 79 / 75 us with one / two / three and five tokens
+// over them 102 / 97 / 89, but even ones lose by it (2 x 16384 keys of 8 heads of 128 33 / 37 / 39). With at least 4 / 8
+// tiles a split: 4000 keys 14.2 / 16.4 us, 1500 keys 12.4 / 13.9.
 bool choose(const ajib_attn *op, Choice &c)
 {
     const int64_t group = op->hq / op->hk, base = (int64_t)op->batch * op->hk;

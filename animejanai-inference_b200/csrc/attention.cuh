@@ -9,13 +9,11 @@
  */
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <climits>
 #include <cstdint>
 
 #include "../../include/aji_b200.h"
+#include "half_types.cuh"
 
 namespace ajib {
 
@@ -37,12 +35,6 @@ struct AttnDev {
 namespace dev {
 
 constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 __device__ __forceinline__ float exp2_fast(float x)
 {

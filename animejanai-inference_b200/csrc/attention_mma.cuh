@@ -1,7 +1,8 @@
 /*
  * attention_mma.cuh — attention on warp-level tensor instructions (mma.sync m16n8k16, fp32
- * accumulators): small heads and windows, few queries over many keys, and every head size, stride
- * and alignment that the tcgen05 kernel does not take.
+ * accumulators): heads of more than 128 components, layouts that TMA does not copy, documents with few
+ * queries and clamped grid tables; what attention_tc.cuh and attention_few.cuh do not take. Probabilities are
+ * rounded to the type of v, which the instruction wants of both operands; their sum is of the unrounded ones.
  *
  * Rows of a tile are (query, head of the group) pairs, row = query * group + head, so that the heads
  * that share keys share their reads. A block of 4 warps walks the keys in tiles of 64, copied ahead
@@ -36,9 +37,10 @@ struct MmaDev {
 
 namespace dev {
 
-// mbar_wait with a hint (10 us) of how long the hardware may keep a waiting thread asleep: the roles of
-// this kernel wait for one another most of the time, and polling took their issue slots. tiles: how many key
-// tiles (at most 2.2 us each) may rightly come between, for which 40 us each are added to the 2 s.
+// mbar_wait with a hint (10 us) of how long the hardware may keep a waiting thread asleep: the roles of the
+// pipelined kernels (attention_tc.cuh, attention_few.cuh) wait for one another most of the time, and polling took
+// their issue slots. tiles: how many key tiles (at most 2.2 us each) may rightly come between, for which 40 us each
+// are added to the 2 s.
 __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, int *err, int code, int tiles = 0)
 {
     if (mbar_test_wait(bar, parity)) return true;

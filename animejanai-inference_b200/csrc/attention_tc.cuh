@@ -16,14 +16,16 @@
  * The running maximum a row is scaled by only follows the true one when that has grown by more than
  * 2^8: the outputs are rescaled rarely, by the softmax threads themselves, at a time when no product
  * touches them. Probabilities are then up to 2^8 instead of 1, which costs neither fp16 nor bf16 any
- * precision.
+ * precision. They are rounded to the type of v, which the product wants of both operands (against fp32
+ * probabilities a third more error at most, fp16 2.8e-4 and bf16 2.2e-3 of the outputs' size); their sum is of
+ * the unrounded ones.
  *
  * What bounds it: per 256 x 128 scores the tensor pipe needs 32 * DP cycles (8192 flop a cycle) and the
  * exponentials 2048 (16 a cycle): even at DP 128, where 4096 x 4096 tokens of 16 heads take 120 us (1.14
  * PFLOP/s, 69 % of the measured matrix rate) and an 8192-token causal prompt 222 us (1.25 PFLOP/s of
- * the pairs that are seen; events, idle card). At DP 64 it is the instructions of the softmax:
- * about ten an element with a table's bias, half of the issue slots of an SM (2040 windows of 256 tokens, 6
- * heads of 32: 597 us; 20 % of the exponential unit, 23 % of DRAM).
+ * the pairs that are seen; events, idle card). At DP 64 it is the instructions of the softmax: 11 an element
+ * with a table's bias and region masks, half of the issue slots of an SM (2040 windows of 256 tokens, 6 heads of
+ * 32: 550 us; 32 % of the exponential unit, 28 % of DRAM).
  *
  * Tried and left out: taking turns at the exponential unit, a quarter of the exponentials as a polynomial
  * on the FMA pipe (233 against 222 us together, they pay only while products wait for one another);

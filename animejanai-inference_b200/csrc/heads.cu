@@ -12,8 +12,6 @@
  * product wraps whole turns off by itself and the top 32 bits are the angle to 2^-32 of a turn
  * (error below position * 2^-65 turns), for negative positions too.
  */
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -21,6 +19,7 @@
 #include <new>
 
 #include "f32x2.cuh"
+#include "half_types.cuh"
 #include "heads.h"
 
 struct ajib_rotary {
@@ -31,7 +30,13 @@ struct ajib_rotary {
 };
 
 namespace ajib {
+
+int sm_count();  // conv.cu
+
 namespace {
+
+using dev::from_f;
+using dev::to_f;
 
 constexpr int kQkThreads = 128;
 
@@ -51,12 +56,6 @@ struct QkDev {
     float eps, amplitude, inv_d, inv_eps;
     uint64_t turns[kMaxHeadDim / 2];
 };
-
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 // What a position's pairs turn by: itself, or its row and column.
 struct Place {
@@ -249,10 +248,10 @@ enum { kTurnNone = 0, kTurnHalf = 1, kTurnInterleaved = 2 };
 // and of their second, so that pairs meet in a lane; otherwise chunk g of a half of what there is, or two
 // in a row where that does not divide. A lane computes its CS angles once and walks the heads of its token,
 // `split` groups to a token so that small batches fill the machine too. With a norm a head is in
-// flight at a time (64 to 72 registers, 7 or 8 blocks an SM: the sum's and the square root's latency is hidden by other
-// warps), without one two (80 registers, 6 blocks). Measured, one / two heads: norms of 2040 windows 149 /
-// 158 us, norms and rotation of 8192 tokens 46 / 50, rotation alone of 2 x 4999 tokens 39 / 39, of 8 frames
-// of 8160 76 / 70.
+// flight at a time (60 to 72 registers, 7 or 8 blocks an SM: other warps hide the latency of the sum and
+// the root), without one two (80 registers, 6 blocks). Measured, one / two heads: norms of 2040 windows
+// 171 / 172 us, norms and rotation of 8192 tokens 43.3 / 41.0, rotation alone of 2 x 4999 tokens 42.3 / 38.9,
+// of 8 frames of 8160 73.7 / 69.6. (With a norm 44 to 54 % of issue slots and about as much of DRAM: neither is full.)
 // WHOLE: every component turns, or none, and the head divides into pairs of chunks, which spares the
 // lanes the question (norms and rotation of 8192 tokens 30 M instructions, 49 us, without it).
 template <typename T, int CS, bool NORM, int TURN, bool WHOLE>
@@ -432,7 +431,7 @@ cudaError_t run_qk(QkDev &p, int width, int64_t rows, cudaStream_t s)
         // groups of lanes to a token: one does all its heads once that gives every SM 2048 lanes; a divisor
         // of both head counts, so that no group idles, if one is near (40 heads of 8192 tokens: 4 groups
         // 45.6 us, 5 53.5)
-        const int64_t lanes = rows * g, want = 148 * 2048;
+        const int64_t lanes = rows * g, want = (int64_t)sm_count() * 2048;
         p.split = (int)std::min<int64_t>(heads, std::max<int64_t>(1, (want + lanes - 1) / lanes));
         if (p.split < heads)
             for (int s = p.split; 2 * s >= p.split; s--)

@@ -340,7 +340,7 @@ AJIB_EXPORT int ajib_exec_info(const ajib_exec *e, size_t *device_bytes, size_t 
  * element at p + b * sb + t * st + h * sh + i (strides in elements, not negative; components are
  * contiguous). A fused projection's queries, keys and values are three of these over one buffer, a
  * cache is one whose st is its row. Inputs may repeat (stride 0); the elements of an output must be
- * distinct (AJIB_ERR_ARGS otherwise). Pointers need the element's 2-byte alignment; with 16-byte
+ * distinct, in nested strides: each past all that the smaller ones span (AJIB_ERR_ARGS otherwise). Pointers need the element's 2-byte alignment; with 16-byte
  * aligned pointers and strides that are multiples of 8 the widest copies are used. */
 enum ajib_dtype { AJIB_F16 = 0, AJIB_BF16 = 1 };
 typedef struct ajib_heads {
@@ -412,7 +412,9 @@ AJIB_EXPORT int ajib_qk_launch(const ajib_qk *op, const ajib_heads *q, const aji
 /* Attention of queries q over keys k and values v, softmax over the keys each query sees:
  *   s = scale * q . k;  s = cap * tanh(s / cap) (cap > 0);  s += bias;  out = softmax(s) v
  * Query head h reads key and value head h / (hq / hk) (hq a multiple of hk). Scores, softmax and
- * sums are fp32; the probabilities are rounded to the type of v before their product with v.
+ * sums are fp32; the probabilities are rounded to the type of v before their product with v. They are
+ * divided by their sum at the end, and may be up to 2^8 before: values (bf16) of 2^119 divided by the
+ * number of keys, and larger ones, can leave fp32's range on the way.
  *
  * Where queries stand: key j of a sequence stands at j; query i stands at i, or with align_end at
  * i + (keys - queries) of its sequence, so that the last query stands at the last key (new tokens
