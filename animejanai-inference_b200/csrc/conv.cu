@@ -90,9 +90,12 @@ int *status_word()
 
 int sm_count()
 {
+    static std::atomic<int> counts[64] = {};  // (asked for in every launch)
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 148;
+    if (dev < 64 && (n = counts[dev].load(std::memory_order_relaxed))) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (dev < 64) counts[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
