@@ -182,3 +182,42 @@ def test_time_of_a_long_prompt(d, keys, most):
     assert torch.isfinite(out[..., 1:]).all()
     print(f"{clean:.0f} us, {slow:.0f} us")
     assert slow < most * clean, f"{clean:.0f} us without, {slow:.0f} us with"
+
+
+@pytest.mark.parametrize("hq,hk", [(20, 1), (12, 4), (64, 2)])
+@pytest.mark.parametrize("lq,lk", [(1, 300), (3, 2000), (9, 300), (140, 140)])
+@pytest.mark.parametrize("d", [64, 128, 160])
+def test_shared_heads(hq, hk, lq, lk, d):
+    """16 rows of a group's heads and several queries, whose last ones see the key and whose first do not."""
+    q, k, v = with_odd("bf16", 2, lq, lk, hq, hk, d, [lk - 2, lk - 1], math.inf, component=d // 2, fused=False)
+    run(q, k, v, causal=True, align_end=True)
+    run(q, k, v, causal=True, align_end=True, left=70, k_len=[lk, lk - 1])
+
+
+@pytest.mark.parametrize("d,lq,lk", [(64, 300, 300), (128, 300, 300), (30, 300, 300), (128, 2, 5000), (160, 200, 200)])
+def test_replays(d, lq, lk):
+    """A captured call whose values become finite, and not, between replays; the same bits each time."""
+    import ajib
+    q, k, v = (x.clone() for x in make("f16", 2, lq, lk, 12, 12, d))
+    out = torch.zeros_like(q)
+    op = ajib.attn_op(ajib.F16, 2, lq, lk, 12, 12, d, 0.1, causal=True, align_end=True, left=2000)
+    n = ajib.attention_workspace(op)
+    space = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    heads = [ajib.heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)) for t in (q, k, v, out)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        assert ajib.attention(op, *heads, space.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
+    clean = v.clone()
+    for odd in (None, math.nan, None, -math.inf):
+        v.copy_(clean)
+        if odd is not None:
+            v[0, lk - 70, :, 3] = odd
+            v[1, lk - 1, ::2] = odd
+        outs = []
+        for _ in range(2):
+            out.fill_(7.0)
+            g.replay()
+            torch.cuda.synchronize()
+            outs.append(out.clone())
+        assert torch.equal(outs[0].view(torch.int16), outs[1].view(torch.int16)) and ajib.kernel_status() == 0
+        assert_attention(out, *definition(q, k, v, scale=0.1, causal=True, align_end=True, left=2000))
