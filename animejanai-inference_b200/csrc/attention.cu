@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 
 #include "attention_few.cuh"
@@ -263,6 +264,12 @@ extern "C" int ajib_attention_launch(const ajib_attn *op, const ajib_heads *q, c
     if (op->lk) {
         if (!heads_ok(k, b, op->lk, op->hk, d) || !heads_ok(v, b, op->lk, op->hk, d)) return AJIB_ERR_ARGS;
         if (out->p == k->p || out->p == v->p) return AJIB_ERR_ARGS;
+    }
+    ajib_attn uncapped;
+    if (op->cap > 0 && std::fabs(op->scale / op->cap) < FLT_MIN) {  // (a subnormal loses bits; tanh is its argument here)
+        uncapped = *op;
+        uncapped.cap = 0;
+        op = &uncapped;
     }
     Choice c;
     if (!choose(op, c)) return AJIB_ERR_UNSUPPORTED;

@@ -17,7 +17,7 @@
  * kernel has 80 registers), most of it the instructions of one warp and their fetches: a question asked at run time
  * around each load (aligned or not) made it 7000. 8192 causal tokens, 16 heads of 64 / 128, 250 us: with a NaN in
  * the first key 400 / 540 us, in key 4000 800 / 760, in the last 1900 / 1400, with nothing finite behind the first
- * 5.0 / 4.8 ms. (Key by key it was two orders of magnitude for any of them.)
+ * 5.0 / 4.8 ms.
  */
 #pragma once
 

@@ -70,3 +70,12 @@ def test_below_and_above_in_one_tile(d):
         for cap in (2.0, 30.0):
             check(q, k, v, cap=cap)
             check(q, k, v, cap=cap, scale=-0.3, causal=True)
+
+
+@pytest.mark.parametrize("d", [64, 128, 160])
+@pytest.mark.parametrize("cap,scale", [(2e38, 1e-3), (2e38, 0.1), (2e38, 3e-6), (1e38, -1e-6), (1e30, 1e-8)])
+def test_caps_past_every_score(cap, scale, d):
+    """scale / cap is a subnormal number of few bits, or nearly."""
+    for batch, lq, hq in ((1, 3, 2), (6, 200, 12)):
+        q, k, v = make("bf16", batch, lq, 200, hq, hq, d, gain=3.0 * d ** -0.5 / abs(scale), fused=False)
+        check(q, k, v, cap=cap, scale=scale)
